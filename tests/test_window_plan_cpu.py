@@ -1,0 +1,34 @@
+"""Tile plan of the window attention kernels (csrc/window_plan.h), compiled for the host and checked against the definition."""
+import os
+import random
+import shutil
+import subprocess
+
+import pytest
+
+import train_large_model_from_scratch_b200 as pkg
+
+SRC = os.path.join(os.path.dirname(pkg.__file__), "csrc")
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    if shutil.which("g++") is None:
+        pytest.skip("no host compiler")
+    exe = str(tmp_path_factory.mktemp("plan") / "plan")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", SRC, os.path.join(HERE, "window_plan_host_test.cpp"), "-o", exe], check=True)
+    return exe
+
+
+def test_every_visible_pair_is_met_once(plan):
+    rng = random.Random(0)
+    sizes = [1, 2, 127, 128, 129, 255, 256, 257, 640, 1001]
+    cases = [(T, W, S) for T in sizes for W in sizes if W <= T for S in (0, 1, 4, 127, 128, 129, 300, 1001) if S <= T]
+    for _ in range(100):
+        T = rng.randint(1, 2000)
+        cases.append((T, rng.randint(1, T), rng.choice([0, rng.randint(0, min(T, 20)), rng.randint(0, T)])))
+    cases += [(4000, 1, 1), (4000, 128, 4), (4000, 1000, 500)]
+    out = subprocess.run([plan], input="".join("%d %d %d\n" % c for c in cases), capture_output=True, text=True, check=True).stdout.split("\n")
+    bad = [(c, o) for c, o in zip(cases, out) if o != "ok"]
+    assert len(out) == len(cases) + 1 and not bad, bad[:5]

@@ -23,12 +23,18 @@
 // A second instantiation of the main kernel (SCATTER) serves Ulysses sequence parallelism: its dK / dV epilogue
 // rotates dK itself and stores the rows straight into the sequence owners' packed gradient buffers, and the
 // conversion pass does the same for dQ.
+// A third one (WIN) takes a sliding window with sinks (window_plan.h) and q, k, v and their gradients as tensors of their own: a block
+// walks over the query tiles of its KV tile's window; the query tiles that see a tile only as sinks are further blocks, whose
+// dV | dK rows meet the tile's own in an fp32 buffer that the conversion pass adds up in fixed order.
 // Every wait is bounded; on a timeout the CTA records a status code, leaves its
 // loops and still releases its tensor memory.
 #include "common.cuh"
+#include "window_plan.h"
 #include <cstdlib>
 
 namespace tlm {
+
+int make_bthd_map(CUtensorMap* map, const void* base, const long long* strides, int B, int T, int heads, int hd, int box_rows, int box_cols);
 
 constexpr int AB_TILE = 128, AB_THREADS = 704, AB_MAX_DST = 8;
 
@@ -60,7 +66,18 @@ struct AttnBwdParams {
   int n_dst, dst_rows, dst_heads, dst_q0, dst_k0, dst_v0;
   int split;               // SPLIT instantiation: CTAs of the cluster that share one KV tile's steps
   int head_group;          // (batch, KV head) pairs per group of the heavy-first block order (see heavy_first_decode)
+  // WIN instantiation only
+  int window, sinks;       // in [1, T], [0, T]
+  WinFar far;
+  float* part;             // far.chunks > 0: [B Hkv][1 + far.chunks][sinks][dV HD | dK HD], of tiles below far.tiles; slot 0: the window's
+  const __nv_bfloat16 *k, *v;
+  __nv_bfloat16 *dk, *dv;
+  long long ks[3], vs[3], dks[3], dvs[3];      // batch, token, head strides in elements
 };
+
+// WIN: q [.., Hq, hd], k and v [.., Hkv, hd]; else one map over the packed tensor
+template <bool WIN> struct AttnBwdMaps { CUtensorMap qkv, dout, dq; };
+template <> struct AttnBwdMaps<true> { CUtensorMap q, k, v, dout, dq; };
 
 // delta[b, h, t] = sum_c o[b, t, h, c] * dout[b, t, h, c]. One block per (b, 32 consecutive t): that slab of o
 // and dout is contiguous, hd / 8 lanes share a row with 16-byte loads (four rows in flight per lane), the row sums
@@ -190,6 +207,80 @@ __global__ void attn_dq_convert_kernel(const float* dq_acc, __nv_bfloat16* __res
   }
 }
 
+// The window's conversion: rows of dQ (fp32 accumulator * scale -> bf16), with `rot` the transposed rotation on the way, then the
+// rows of dK and dV that the main kernel has not finished: with `rot` all of dK (bf16, in place), and the sink rows of dK and dV,
+// whose fp32 parts are added up slot by slot. An item is 8 low columns and their 8 partners (j + hd / 2) of a row.
+struct AttnWinFinish {
+  const float* dq_acc;
+  const float* part;                 // see AttnBwdParams
+  __nv_bfloat16 *dq, *dk, *dv;
+  long long dqs[3], dks[3], dvs[3];
+  const float *cosT, *sinT;
+  int B, T, Hq, Hkv, hd;
+  int sinks, slots, slot_rows;       // rows whose sums are in `part`, its slots and a slot's rows
+  int k_rows, v_rows;                // rows of a dK / dV head that are items: T with a rotation, the sinks, or none
+  float scale;
+};
+
+__global__ void __launch_bounds__(256)
+attn_window_finish_kernel(const AttnWinFinish p) {
+  griddep_wait();
+  griddep_launch();
+  const int half = p.hd / 2, vec_log = p.hd == 32 ? 1 : p.hd == 64 ? 2 : 3;          // hd / 16 items per row
+  const long long q_rows = (long long)p.B * p.Hq * p.T, k_all = (long long)p.B * p.Hkv * p.k_rows;
+  const long long total = (q_rows + k_all + (long long)p.B * p.Hkv * p.v_rows) << vec_log;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const int j = (int)(i & ((1 << vec_log) - 1)) * 8;
+    long long r = i >> vec_log;
+    const int kind = r < q_rows ? 0 : r < q_rows + k_all ? 1 : 2;               // dQ, dK, dV
+    if (kind > 0) r -= kind == 1 ? q_rows : q_rows + k_all;
+    const int rows = kind == 0 ? p.T : kind == 1 ? p.k_rows : p.v_rows, heads = kind == 0 ? p.Hq : p.Hkv;
+    const int bh = (int)(r / rows), t = (int)(r - (long long)bh * rows), b = bh / heads, h = bh - b * heads;
+    __nv_bfloat16* dst = kind == 0 ? p.dq + b * p.dqs[0] + t * p.dqs[1] + h * p.dqs[2]
+                       : kind == 1 ? p.dk + b * p.dks[0] + t * p.dks[1] + h * p.dks[2] : p.dv + b * p.dvs[0] + t * p.dvs[1] + h * p.dvs[2];
+    dst += j;
+    float lo[8], hi[8];
+    if (kind == 0 || (p.part != nullptr && t < p.sinks)) {
+      const float* src = kind == 0 ? p.dq_acc + ((long long)bh * p.T + t) * p.hd + j
+                                   : p.part + ((long long)bh * p.slots * p.slot_rows + t) * (2 * p.hd) + (kind == 1 ? p.hd : 0) + j;
+      const long long slot = (long long)p.slot_rows * 2 * p.hd;
+      const float osc = kind == 2 ? 1.f : p.scale;
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
+        *reinterpret_cast<float4*>(lo + k) = *reinterpret_cast<const float4*>(src + k);
+        *reinterpret_cast<float4*>(hi + k) = *reinterpret_cast<const float4*>(src + half + k);
+      }
+      if (kind > 0)
+        for (int n = 1; n < p.slots; ++n) {
+          const float* s = src + n * slot;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) { lo[k] += s[k]; hi[k] += s[half + k]; }
+        }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { lo[k] *= osc; hi[k] *= osc; }
+    } else {                                             // a finished row of dK, to be rotated
+      const uint4 a = *reinterpret_cast<const uint4*>(dst), c = *reinterpret_cast<const uint4*>(dst + half);
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 x = unpack_bf16(aw[k]), y = unpack_bf16(cw[k]);
+        lo[2 * k] = x.x; lo[2 * k + 1] = x.y; hi[2 * k] = y.x; hi[2 * k + 1] = y.y;
+      }
+    }
+    if (p.cosT != nullptr && kind < 2) {
+      const float *c = p.cosT + (long long)t * p.hd + j, *sn = p.sinT + (long long)t * p.hd + j;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float a = lo[k], bb = hi[k];
+        lo[k] = a * c[k] + bb * sn[half + k];
+        hi[k] = bb * c[half + k] - a * sn[k];
+      }
+    }
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
+    *reinterpret_cast<uint4*>(dst + half) = make_uint4(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]), pack_bf16(hi[4], hi[5]), pack_bf16(hi[6], hi[7]));
+  }
+}
+
 // What a step consists of, and what bounds it. Every step is taken in two halves of 64 query columns, each with its own eight
 // softmax warps and barriers: while one half's exponentials run, the other half's products do. For head dims 32 and 64 there
 // are three score tiles for the two halves, so a half's scores of its next step are there before its warps ask for them
@@ -242,8 +333,9 @@ struct AttnBwdCfg {
 
 // P of 32 query columns of one KV row: scores from tensor memory, -lse of the columns from shared memory; columns below
 // `masked` come before the row (DIAG).
-template <bool DIAG>
-__device__ __forceinline__ void attn_bwd_p(uint32_t t_s, const float* nlse, float2 sc2, int masked, float2* pr) {
+// WIN (with DIAG): columns [masked, masked + width) are seen.
+template <bool DIAG, bool WIN = false>
+__device__ __forceinline__ void attn_bwd_p(uint32_t t_s, const float* nlse, float2 sc2, int masked, float2* pr, uint32_t width = 0) {
 #pragma unroll
   for (int c = 0; c < 32; c += 16) {
     uint32_t sv[16];
@@ -257,7 +349,12 @@ __device__ __forceinline__ void attn_bwd_p(uint32_t t_s, const float* nlse, floa
       float2* o = pr + ((c + i) >> 1);
       o[0] = make_float2(ex2_approx(x.x), ex2_approx(x.y));
       o[1] = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-      if (DIAG) {
+      if (WIN) {
+        if ((uint32_t)(c + i - masked) >= width) o[0].x = 0.f;
+        if ((uint32_t)(c + i + 1 - masked) >= width) o[0].y = 0.f;
+        if ((uint32_t)(c + i + 2 - masked) >= width) o[1].x = 0.f;
+        if ((uint32_t)(c + i + 3 - masked) >= width) o[1].y = 0.f;
+      } else if (DIAG) {
         if (c + i < masked) o[0].x = 0.f;
         if (c + i + 1 < masked) o[0].y = 0.f;
         if (c + i + 2 < masked) o[1].x = 0.f;
@@ -269,10 +366,10 @@ __device__ __forceinline__ void attn_bwd_p(uint32_t t_s, const float* nlse, floa
 
 // SPLIT: a cluster of p.split CTAs works on one KV tile, each on its share of the (query head, query tile) steps; every CTA
 // leaves its fp32 dV | dK in its own shared memory and the cluster adds them up, in fixed order. See split_for.
-template <int HD, bool SCATTER, bool SPLIT>
+template <int HD, bool SCATTER, bool SPLIT, bool WIN>
 __global__ void __launch_bounds__(AB_THREADS, 1)
-attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
-                const __grid_constant__ CUtensorMap tm_dq, const AttnBwdParams p) {
+attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams p) {
+  static_assert(!(WIN && SCATTER), "the window has no head -> sequence return");
   using C = AttnBwdCfg<HD>;
   constexpr uint32_t TMEM_COLS = 512;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -295,22 +392,49 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
   const int n_tiles = (p.T + AB_TILE - 1) / AB_TILE;
   int j, bh;                                                  // KV tile (tile 0 has the most query tiles), (batch, KV head)
   const int split = SPLIT ? p.split : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
-  heavy_first_decode((int)blockIdx.x / split, n_tiles, p.B * p.Hkv, p.head_group, j, bh);
+  int q_from, q_to, part = -1;                                // query tiles; slot of `part` that this block's sink rows go to
+  if constexpr (WIN) {
+    // the far pieces first: they are as long as the others, and the last blocks should not be theirs
+    const int item = (int)blockIdx.x / split, far_items = p.far.tiles * p.far.chunks * p.B * p.Hkv;
+    if (item < far_items) {
+      const int c = item % p.far.chunks, r = item / p.far.chunks;
+      j = r % p.far.tiles;
+      bh = r / p.far.tiles;
+      win_far_range(p.far, j, c, p.window, n_tiles, q_from, q_to);
+      part = 1 + c;
+    } else {
+      heavy_first_decode(item - far_items, n_tiles, p.B * p.Hkv, p.head_group, j, bh);
+      q_from = j;
+      q_to = win_last_q(j, p.window, n_tiles) + 1;
+      if (j < p.far.tiles) part = 0;
+    }
+  } else {
+    heavy_first_decode((int)blockIdx.x / split, n_tiles, p.B * p.Hkv, p.head_group, j, bh);
+    q_from = j;                                               // query tiles j..n_tiles-1
+    q_to = n_tiles;
+  }
   const int b = bh / p.Hkv, kvh = bh % p.Hkv;
   const int rep = p.Hq / p.Hkv;
-  const int per_head = n_tiles - j;                           // query tiles j..n_tiles-1
+  const int per_head = WIN && q_to < q_from ? 0 : q_to - q_from;
   const int it0 = SPLIT ? rep * per_head * rank / split : 0;                                       // this CTA's steps
   const int n_it = SPLIT ? rep * per_head * (rank + 1) / split - it0 : rep * per_head;             // (SPLIT: may be none)
   const int heads_total = p.Hq + 2 * p.Hkv;
+  const CUtensorMap *tm_q, *tm_k, *tm_v;
+  int k_head = kvh, v_head = kvh;
+  if constexpr (WIN) { tm_q = &tm.q; tm_k = &tm.k; tm_v = &tm.v; }
+  else { tm_q = tm_k = tm_v = &tm.qkv; k_head += p.Hq; v_head += p.Hq + p.Hkv; }
+  // fp32 row of slot `part` for key t (dV, then dK)
+  auto part_row = [&](int t) { return p.part + (((long long)bh * (1 + p.far.chunks) + part) * p.sinks + t) * (2 * HD); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < N_BARS; ++i)
       mbar_init(bar(i), i == KV_TMEM ? 16 : (i == PDS || i == PDS + 1) ? 8 : i == DQ_FREE ? 4 : (i >= RING_FULL && i < RING_EMPTY) ? 2 : 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tm_qkv);
-    tma_prefetch_desc(&tm_do);
-    tma_prefetch_desc(&tm_dq);
+    tma_prefetch_desc(tm_q);
+    if (WIN) { tma_prefetch_desc(tm_k); tma_prefetch_desc(tm_v); }
+    tma_prefetch_desc(&tm.dout);
+    tma_prefetch_desc(&tm.dq);
   }
   if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
   tc_fence_before();
@@ -325,20 +449,20 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
       mbar_expect_tx(bar(KV_FULL), (C::KV_TMEM ? 1 : 2) * C::TILE_BYTES);
 #pragma unroll
       for (int kb = 0; kb < C::KB; ++kb) {
-        tma_load_4d(sbase + C::OFF_K + kb * 16384, &tm_qkv, bar(KV_FULL), kb * 64, p.Hq + kvh, j * AB_TILE, b);
-        if (!C::KV_TMEM) tma_load_4d(sbase + C::OFF_V + kb * 16384, &tm_qkv, bar(KV_FULL), kb * 64, p.Hq + p.Hkv + kvh, j * AB_TILE, b);
+        tma_load_4d(sbase + C::OFF_K + kb * 16384, tm_k, bar(KV_FULL), kb * 64, k_head, j * AB_TILE, b);
+        if (!C::KV_TMEM) tma_load_4d(sbase + C::OFF_V + kb * 16384, tm_v, bar(KV_FULL), kb * 64, v_head, j * AB_TILE, b);
       }
     }
     for (int it = 0; it < n_it; ++it) {
       const int st = it % C::STAGES;
-      const int hq = kvh * rep + (it0 + it) / per_head, qi = j + (it0 + it) % per_head;
+      const int hq = kvh * rep + (it0 + it) / per_head, qi = q_from + (it0 + it) % per_head;
       if (!mbar_wait_warp(bar(RING_EMPTY + st), ((uint32_t)(it / C::STAGES) & 1u) ^ 1u, 21, abort_flag, p.status)) break;
       if (lane == 0) {
         mbar_expect_tx(bar(RING_FULL + st), (C::WIDE ? 1 : 2) * C::TILE_BYTES);
 #pragma unroll
         for (int kb = 0; kb < C::KB; ++kb)
-          tma_load_4d(sbase + C::OFF_Q + st * C::TILE_BYTES + kb * 16384, &tm_qkv, bar(RING_FULL + st), kb * 64, hq, qi * AB_TILE, b);
-        if (!C::WIDE) tma_load_4d(sbase + C::OFF_DO + st * C::TILE_BYTES, &tm_do, bar(RING_FULL + st), 0, hq, qi * AB_TILE, b);
+          tma_load_4d(sbase + C::OFF_Q + st * C::TILE_BYTES + kb * 16384, tm_q, bar(RING_FULL + st), kb * 64, hq, qi * AB_TILE, b);
+        if (!C::WIDE) tma_load_4d(sbase + C::OFF_DO + st * C::TILE_BYTES, &tm.dout, bar(RING_FULL + st), 0, hq, qi * AB_TILE, b);
       }
       constexpr float LOG2E = 1.4426950408889634f;
       const long long r0 = ((long long)b * p.Hq + hq) * p.T;
@@ -360,7 +484,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
           mbar_expect_tx(bar(DO_FULL), C::TILE_BYTES);
 #pragma unroll
           for (int kb = 0; kb < C::KB; ++kb)
-            tma_load_4d(sbase + C::OFF_DO + kb * 16384, &tm_do, bar(DO_FULL), kb * 64, hq, qi * AB_TILE, b);
+            tma_load_4d(sbase + C::OFF_DO + kb * 16384, &tm.dout, bar(DO_FULL), kb * 64, hq, qi * AB_TILE, b);
         }
       }
     }
@@ -512,7 +636,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
     if constexpr (C::KV_TMEM) {   // K (warps of half 0) and V (half 1) rows become tensor-memory operands, half a row per warp
       static_assert(HD == 32, "half a row is 16 columns, 8 words; p.hd is HD (the scatter form has wider tiles)");
       const int c0 = (g & 1) * 16;
-      const __nv_bfloat16* src = p.qkv + (((long long)b * p.T + t_row) * heads_total + p.Hq + s * p.Hkv + kvh) * HD + c0;
+      const __nv_bfloat16* src = WIN ? (s == 0 ? p.k + b * p.ks[0] + t_row * p.ks[1] + kvh * p.ks[2] : p.v + b * p.vs[0] + t_row * p.vs[1] + kvh * p.vs[2]) + c0
+                                     : p.qkv + (((long long)b * p.T + t_row) * heads_total + p.Hq + s * p.Hkv + kvh) * HD + c0;
       uint32_t w[8];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -528,7 +653,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     const int col0 = (g & 1) * 32;                             // of the half's 64 query columns
     for (int it = 0; it < n_it; ++it) {
-      const int st = it % C::STAGES, qi = j + (it0 + it) % per_head;
+      const int st = it % C::STAGES, qi = q_from + (it0 + it) % per_head;
       const float* rows = reinterpret_cast<const float*>(sal + C::OFF_ROW) + st * 2 * AB_TILE + s * 64 + col0;
       uint8_t* drow = sal + C::OFF_DS + (C::WIDE ? 0 : it & 1) * C::DS_BYTES + s * 16384 + row * 128;
       if (!mbar_wait_warp(bar(RING_FULL + st), (uint32_t)(it / C::STAGES) & 1u, 28, abort_flag, p.status)) { ok = false; break; }
@@ -538,7 +663,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
       tc_fence_after();
       float2 pr[16];
       // two copies: the compare and select of the diagonal tiles doubled the instructions of a pair in all the others
-      if (qi == j) attn_bwd_p<true>(t_s, rows, sc2, row - s * 64 - col0, pr);
+      if constexpr (WIN) {
+        if (qi == j || ((qi - j) * AB_TILE + AB_TILE - 1 >= p.window && (j + 1) * AB_TILE > p.sinks))
+          attn_bwd_p<true, true>(t_s, rows, sc2, (j - qi) * AB_TILE + row - s * 64 - col0, pr, t_row < p.sinks ? 0x80000000u : (uint32_t)p.window);
+        else attn_bwd_p<false>(t_s, rows, sc2, 0, pr);
+      } else if (qi == j) attn_bwd_p<true>(t_s, rows, sc2, row - s * 64 - col0, pr);
       else attn_bwd_p<false>(t_s, rows, sc2, 0, pr);
       {
         uint32_t pp[16];
@@ -592,6 +721,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
         const float osc = which == 0 ? 1.f : p.scale;
         __nv_bfloat16* dst = p.dqkv + (((long long)b * p.T + t_row) * heads_total + (which == 0 ? p.Hq + p.Hkv : p.Hq) + kvh) * p.hd + out0;
         bool dst_ok = t_row < p.T && out0 < p.hd;
+        float* part_dst = nullptr;
+        if constexpr (WIN) {
+          dst = which == 0 ? p.dv + b * p.dvs[0] + t_row * p.dvs[1] + kvh * p.dvs[2] + out0 : p.dk + b * p.dks[0] + t_row * p.dks[1] + kvh * p.dks[2] + out0;
+          if (part >= 0 && t_row < p.sinks) part_dst = part_row(t_row) + which * HD + out0;
+          else if (part > 0) dst_ok = false;                    // a far piece has nothing for rows behind the sinks
+        }
         if (SCATTER && p.n_dst > 0) {
           const int owner = t_row / p.dst_rows, tl = t_row - owner * p.dst_rows;
           dst_ok = dst_ok && owner < p.n_dst;
@@ -616,7 +751,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
             }
           }
         }
-        if (dst_ok) {
+        if (WIN && part_dst != nullptr) {
+#pragma unroll
+          for (int i = 0; i < W; i += 4)
+            *reinterpret_cast<uint4*>(part_dst + i) = n_it > 0 ? make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]) : make_uint4(0, 0, 0, 0);
+        } else if (dst_ok) {
 #pragma unroll
           for (int i = 0; i < W; i += 8) {
             uint4 v;
@@ -652,7 +791,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
     const uint32_t t_lane = tmem + ((uint32_t)(q4 * 32) << 16);
     const int box0 = C::OFF_DQS + q4 * C::BOXES * 4096;
     for (int it = 0; it < n_it; ++it) {
-      const int hq = kvh * rep + (it0 + it) / per_head, qi = j + (it0 + it) % per_head;
+      const int hq = kvh * rep + (it0 + it) / per_head, qi = q_from + (it0 + it) % per_head;
       const int y0 = qi * AB_TILE + q4 * 32;                  // first of this warp's 32 query rows
       if (!mbar_wait_warp(bar(DQ_FULL + (C::WIDE ? 0 : it & 1)), (uint32_t)(C::WIDE ? it : it >> 1) & 1u, 32, abort_flag, p.status)) break;
       tc_fence_after();
@@ -687,7 +826,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
             for (int x = 0; x < C::BOXES; ++x)
               if (y0 < p.T && c0 + c + 32 * x < p.hd)
                 asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
-                             ::"l"((uint64_t)&tm_dq), "r"(sbase + box0 + x * 4096), "r"(c0 + c + 32 * x), "r"(y0), "r"(b * p.Hq + hq) : "memory");
+                             ::"l"((uint64_t)&tm.dq), "r"(sbase + box0 + x * 4096), "r"(c0 + c + 32 * x), "r"(y0), "r"(b * p.Hq + hq) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         }
@@ -725,10 +864,22 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
       const bool is_k = c >= HD;
       const float osc = is_k ? p.scale : 1.f;
       const float* v = base + r * C::PART_PITCH + c;
+      if constexpr (WIN) {
+        if (part >= 0 && t_row < p.sinks) {
+          float* d = part_row(t_row) + c;                       // dV | dK, as they lie here
+          *reinterpret_cast<float4*>(d) = *reinterpret_cast<const float4*>(v);
+          *reinterpret_cast<float4*>(d + 4) = *reinterpret_cast<const float4*>(v + 4);
+          continue;
+        }
+        if (part > 0) continue;
+      }
       uint4 o;
       o.x = pack_bf16(v[0] * osc, v[1] * osc); o.y = pack_bf16(v[2] * osc, v[3] * osc);
       o.z = pack_bf16(v[4] * osc, v[5] * osc); o.w = pack_bf16(v[6] * osc, v[7] * osc);
-      *reinterpret_cast<uint4*>(p.dqkv + (((long long)b * p.T + t_row) * heads_total + (is_k ? p.Hq : p.Hq + p.Hkv) + kvh) * p.hd + (c - (is_k ? HD : 0))) = o;
+      __nv_bfloat16* dst;
+      if constexpr (WIN) dst = is_k ? p.dk + b * p.dks[0] + t_row * p.dks[1] + kvh * p.dks[2] : p.dv + b * p.dvs[0] + t_row * p.dvs[1] + kvh * p.dvs[2];
+      else dst = p.dqkv + (((long long)b * p.T + t_row) * heads_total + (is_k ? p.Hq : p.Hq + p.Hkv) + kvh) * p.hd;
+      *reinterpret_cast<uint4*>(dst + (c - (is_k ? HD : 0))) = o;
     }
     cluster_sync_all();                // no CTA leaves while another may still read its part
   }
@@ -744,11 +895,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
 // work per SM; its pick was within 1 % of the fastest of 1, 2, 4, 8 on seventeen measured shapes of all head dims. With delta and
 // conversion passes, in us, unsplit -> picked: 1 x 8192, 8 / 1 heads of 64 680 -> 194; 4 x 777, 16 / 2 94 -> 51; 3 x 1001, 12 / 4
 // 50 -> 40; 1 x 1074, 8 / 2 of 128 108 -> 41; 2 x 256, 8 / 2 of 32 20 -> 14.
-static int split_for(int n_tiles, int heads_kv, int rep) {
+// `heaviest`: steps of the longest block, `tiles`: blocks, `total`: steps of all.
+static int split_for(double heaviest, double tiles, double total) {
   const char* v = getenv("TLM_ATTN_BWD_SPLIT");          // 1, 2, 4 or 8: for tests and measurements
   const int forced = v != nullptr ? atoi(v) : 0;
   if (forced == 1 || forced == 2 || forced == 4 || forced == 8) return forced;
-  const double heaviest = (double)rep * n_tiles, tiles = (double)n_tiles * heads_kv, total = heaviest * (n_tiles + 1) / 2 * heads_kv;
   const double sms = num_sms();
   int best = 1;
   double best_cost = heaviest > total / sms ? heaviest : total / sms;
@@ -759,19 +910,39 @@ static int split_for(int n_tiles, int heads_kv, int rep) {
   return best;
 }
 
-template <int HD, bool SCATTER, bool SPLIT = false>
-static int launch_bwd(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMap& mdq, const AttnBwdParams& p,
-                      cudaStream_t st) {
+template <int HD, bool SCATTER, bool SPLIT = false, bool WIN = false>
+static int launch_bwd(const AttnBwdMaps<WIN>& maps, const AttnBwdParams& p, cudaStream_t st) {
   constexpr int smem = AttnBwdCfg<HD>::TOTAL;
-  auto kern = attn_bwd_kernel<HD, SCATTER, SPLIT>;
+  auto kern = attn_bwd_kernel<HD, SCATTER, SPLIT, WIN>;
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
-  const int grid = ((p.T + AB_TILE - 1) / AB_TILE) * p.B * p.Hkv;
-  return launch_overlapped(kern, dim3((unsigned)(grid * (SPLIT ? p.split : 1))), dim3(AB_THREADS), smem, st, SPLIT ? p.split : 1, mq, mdo, mdq, p);
+  const int grid = ((p.T + AB_TILE - 1) / AB_TILE + (WIN ? p.far.tiles * p.far.chunks : 0)) * p.B * p.Hkv;
+  return launch_overlapped(kern, dim3((unsigned)(grid * (SPLIT ? p.split : 1))), dim3(AB_THREADS), smem, st, SPLIT ? p.split : 1, maps, p);
+}
+
+// fp32 [B*Hq, T, hd] accumulator, box 32 x 32 x 1
+static int make_dq_map(CUtensorMap* map, const float* dq_acc, int B, int T, int Hq, int hd) {
+  uint64_t dims[3] = {(uint64_t)hd, (uint64_t)T, (uint64_t)B * Hq};
+  uint64_t strides[2] = {(uint64_t)hd * 4, (uint64_t)T * hd * 4};
+  uint32_t box[3] = {32, 32, 1};
+  return make_tmap_f32(map, dq_acc, 3, dims, strides, box);
+}
+
+// delta [B, Hq, T] and a dQ accumulator of zeros
+static int launch_delta(const void* o, const void* dout, float* delta, float* dq_acc, int B, int T, int Hq, int hd, cudaStream_t st) {
+  // Few blocks would take longer over the zeroes than a memset (48 heads of 64, 16 rows: one block, 3 us more)
+  const int delta_blocks = B * ((T + DELTA_T - 1) / DELTA_T);
+  const bool fused_zero = delta_blocks >= num_sms();
+  if (!fused_zero) {
+    const cudaError_t ce = cudaMemsetAsync(dq_acc, 0, (size_t)B * T * Hq * hd * 4, st);
+    if (ce != cudaSuccess) return (int)ce;
+  }
+  return launch_overlapped(attn_delta_kernel, dim3(delta_blocks), dim3(DELTA_THREADS), (size_t)Hq * (DELTA_T + 1) * 4, st, 1,
+      (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, delta, fused_zero ? dq_acc : nullptr, B, T, Hq, hd);
 }
 
 }  // namespace tlm
@@ -788,21 +959,13 @@ static int attn_bwd_impl(const void* qkv, const void* o, const void* dout, const
   if (hd != 32 && hd != 64 && hd != 128) return -4;
   if (Hq % Hkv != 0) return -5;
   if ((size_t)Hq * (DELTA_T + 1) * 4 > 48 * 1024) return -6;
-  // Few blocks would take longer over the zeroes than a memset (48 heads of 64, 16 rows: one block, 3 us more)
-  const int delta_blocks = B * ((T + DELTA_T - 1) / DELTA_T);
-  const bool fused_zero = delta_blocks >= num_sms();
-  if (!fused_zero) {
-    const cudaError_t ce = cudaMemsetAsync(dq_acc, 0, (size_t)B * T * Hq * hd * 4, st);
-    if (ce != cudaSuccess) return (int)ce;
-  }
-  int le = launch_overlapped(attn_delta_kernel, dim3(delta_blocks), dim3(DELTA_THREADS), (size_t)Hq * (DELTA_T + 1) * 4, st, 1,
-      (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, delta, fused_zero ? dq_acc : nullptr, B, T, Hq, hd);
+  const int le = launch_delta(o, dout, delta, dq_acc, B, T, Hq, hd, st);
   if (le) return le;
-  CUtensorMap mq, mdo;
+  AttnBwdMaps<false> maps;
   const int box_cols = hd == 32 && n_dst == 0 ? 32 : 64;
-  int e = make_qkv_map(&mq, qkv, B, T, Hq + 2 * Hkv, hd, AB_TILE, box_cols);
+  int e = make_qkv_map(&maps.qkv, qkv, B, T, Hq + 2 * Hkv, hd, AB_TILE, box_cols);
   if (e) return e;
-  e = make_qkv_map(&mdo, dout, B, T, Hq, hd, AB_TILE, box_cols);
+  e = make_qkv_map(&maps.dout, dout, B, T, Hq, hd, AB_TILE, box_cols);
   if (e) return e;
   if ((cosT == nullptr) != (sinT == nullptr)) return -6;
   if (n_dst < 0 || n_dst > AB_MAX_DST || (n_dst > 0 && (dst_ptrs == nullptr || dst_rows <= 0 || (long long)dst_rows * n_dst < T)))
@@ -820,21 +983,15 @@ static int attn_bwd_impl(const void* qkv, const void* o, const void* dout, const
   AttnBwdDst dd{};
   dd.n = n_dst; dd.rows = dst_rows; dd.heads = dst_heads;
   for (int i = 0; i < n_dst; ++i) { p.dst[i] = (__nv_bfloat16*)dst_ptrs[i]; dd.p[i] = p.dst[i]; }
-  CUtensorMap mdq;                                     // fp32 [B*Hq, T, hd] accumulator, box 32 x 32 x 1
-  {
-    uint64_t dims[3] = {(uint64_t)hd, (uint64_t)T, (uint64_t)B * Hq};
-    uint64_t strides[2] = {(uint64_t)hd * 4, (uint64_t)T * hd * 4};
-    uint32_t box[3] = {32, 32, 1};
-    e = make_tmap_f32(&mdq, dq_acc, 3, dims, strides, box);
-    if (e) return e;
-  }
-  if (n_dst > 0) e = hd == 128 ? launch_bwd<128, true>(mq, mdo, mdq, p, st) : launch_bwd<64, true>(mq, mdo, mdq, p, st);
+  e = make_dq_map(&maps.dq, dq_acc, B, T, Hq, hd);
+  if (e) return e;
+  if (n_dst > 0) e = hd == 128 ? launch_bwd<128, true>(maps, p, st) : launch_bwd<64, true>(maps, p, st);
   else {
-    p.split = split_for((T + AB_TILE - 1) / AB_TILE, B * Hkv, Hq / Hkv);
-    if (p.split > 1) e = hd == 128 ? launch_bwd<128, false, true>(mq, mdo, mdq, p, st) : hd == 64 ? launch_bwd<64, false, true>(mq, mdo, mdq, p, st)
-                                                                                                   : launch_bwd<32, false, true>(mq, mdo, mdq, p, st);
-    else e = hd == 128 ? launch_bwd<128, false>(mq, mdo, mdq, p, st) : hd == 64 ? launch_bwd<64, false>(mq, mdo, mdq, p, st)
-                                                                                : launch_bwd<32, false>(mq, mdo, mdq, p, st);
+    const double n_tiles = (T + AB_TILE - 1) / AB_TILE, rep = Hq / Hkv;
+    p.split = split_for(rep * n_tiles, n_tiles * B * Hkv, rep * n_tiles * (n_tiles + 1) / 2 * B * Hkv);
+    if (p.split > 1) e = hd == 128 ? launch_bwd<128, false, true>(maps, p, st) : hd == 64 ? launch_bwd<64, false, true>(maps, p, st)
+                                                                                           : launch_bwd<32, false, true>(maps, p, st);
+    else e = hd == 128 ? launch_bwd<128, false>(maps, p, st) : hd == 64 ? launch_bwd<64, false>(maps, p, st) : launch_bwd<32, false>(maps, p, st);
   }
   if (e) return e;
   // without a return scatter the main kernel has written un-rotated dK into dqkv: this pass rotates it in place
@@ -861,4 +1018,73 @@ TLM_API int tlm_attn_bwd_scatter(const void* qkv, const void* o, const void* dou
   if (n_dst < 1) return -6;
   return attn_bwd_impl(qkv, o, dout, lse, nullptr, dq_acc, delta, B, T, Hq, Hkv, hd, scale, cosT, sinT, dst_ptrs, n_dst,
                        dst_rows, dst_heads, dst_q0, dst_k0, dst_v0, st);
+}
+
+// Floats of `part` that tlm_attn_window_bwd needs (0: none).
+TLM_API long long tlm_attn_window_part_floats(int B, int T, int Hkv, int hd, int window, int sinks) {
+  if (T <= 0 || T > (1 << 30)) return 0;
+  const int S = sinks < T ? sinks : T;
+  const WinFar f = win_far(T, window > 0 && window < T ? window : T, S);
+  return f.chunks > 0 ? (long long)B * Hkv * (1 + f.chunks) * S * 2 * hd : 0;
+}
+
+// Backward of tlm_attn_window_fwd. strides[9] as there; out_strides[9]: of dq, dk and dv (rows of 16-byte aligned addresses). o, dout
+// [B, T, Hq, hd] and lse contiguous. Scratch owned by the caller: dq_acc, delta as for tlm_attn_bwd, part (see above; may be null
+// where it takes no floats). cosT / sinT (optional, fp32 [T, hd]): the transposed rotation of dQ and dK on the way out.
+TLM_API int tlm_attn_window_bwd(const void* q, const void* k, const void* v, const long long* strides, const void* o, const void* dout,
+                                const float* lse, void* dq, void* dk, void* dv, const long long* out_strides, float* dq_acc, float* delta,
+                                float* part, int B, int T, int Hq, int Hkv, int hd, float scale, const float* cosT, const float* sinT,
+                                int window, int sinks, cudaStream_t st) {
+  if (hd != 32 && hd != 64 && hd != 128) return -4;
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return -5;
+  if ((size_t)Hq * (DELTA_T + 1) * 4 > 48 * 1024) return -6;
+  if (B < 0 || T < 0 || T > (1 << 30) || sinks < 0 || (cosT == nullptr) != (sinT == nullptr)) return -6;
+  if (B == 0 || T == 0) return 0;
+  if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return -7;
+  for (int i = 0; i < 9; ++i) if (out_strides[i] % 8 != 0) return -7;
+  AttnBwdParams p{};
+  p.window = window > 0 && window < T ? window : T;
+  p.sinks = sinks < T ? sinks : T;
+  p.far = win_far(T, p.window, p.sinks);
+  if (p.far.chunks > 0 && part == nullptr) return -6;
+  const double n_tiles = (T + AB_TILE - 1) / AB_TILE, bh = (double)B * Hkv, rep = Hq / Hkv;
+  if ((n_tiles + (double)p.far.tiles * p.far.chunks) * bh * 8 > 2147483647.) return -6;
+  AttnBwdMaps<true> maps;
+  const int cols = hd == 32 ? 32 : 64;
+  const long long o_strides[3] = {(long long)T * Hq * hd, (long long)Hq * hd, hd};
+  int e = make_bthd_map(&maps.q, q, strides, B, T, Hq, hd, AB_TILE, cols);
+  if (!e) e = make_bthd_map(&maps.k, k, strides + 3, B, T, Hkv, hd, AB_TILE, cols);
+  if (!e) e = make_bthd_map(&maps.v, v, strides + 6, B, T, Hkv, hd, AB_TILE, cols);
+  if (!e) e = make_bthd_map(&maps.dout, dout, o_strides, B, T, Hq, hd, AB_TILE, cols);
+  if (!e) e = make_dq_map(&maps.dq, dq_acc, B, T, Hq, hd);
+  if (e) return e;
+  e = launch_delta(o, dout, delta, dq_acc, B, T, Hq, hd, st);
+  if (e) return e;
+  p.dq_acc = dq_acc; p.lse = lse; p.delta = delta; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.hd = hd;
+  p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f; p.status = status_word(); p.part = part;
+  p.k = (const __nv_bfloat16*)k; p.v = (const __nv_bfloat16*)v; p.dk = (__nv_bfloat16*)dk; p.dv = (__nv_bfloat16*)dv;
+  AttnWinFinish f{};
+  for (int i = 0; i < 3; ++i) {
+    p.ks[i] = strides[3 + i]; p.vs[i] = strides[6 + i];
+    f.dqs[i] = out_strides[i]; p.dks[i] = f.dks[i] = out_strides[3 + i]; p.dvs[i] = f.dvs[i] = out_strides[6 + i];
+  }
+  p.head_group = attn_head_group("TLM_ATTN_BWD_GROUP", (long long)T * hd * (10LL * (Hq / Hkv) + 8), 112LL << 20, B * Hkv);
+  // steps: the window's query tiles of every KV tile (fewer at the end), and the far ones of the sink tiles
+  const double wt = win_last_q(0, p.window, (int)n_tiles) + 1, far_items = (double)p.far.tiles * p.far.chunks;
+  const double steps = n_tiles * wt - wt * (wt - 1) / 2 + p.far.tiles * (n_tiles - wt), longest = p.far.chunks > 0 && p.far.chunk > wt ? p.far.chunk : wt;
+  p.split = split_for(rep * longest, (n_tiles + far_items) * bh, rep * steps * bh);
+  if (p.split > 1) e = hd == 128 ? launch_bwd<128, false, true, true>(maps, p, st) : hd == 64 ? launch_bwd<64, false, true, true>(maps, p, st)
+                                                                                               : launch_bwd<32, false, true, true>(maps, p, st);
+  else e = hd == 128 ? launch_bwd<128, false, false, true>(maps, p, st) : hd == 64 ? launch_bwd<64, false, false, true>(maps, p, st)
+                                                                                    : launch_bwd<32, false, false, true>(maps, p, st);
+  if (e) return e;
+  f.dq_acc = dq_acc; f.part = p.far.chunks > 0 ? part : nullptr; f.dq = (__nv_bfloat16*)dq; f.dk = p.dk; f.dv = p.dv;
+  f.cosT = cosT; f.sinT = sinT; f.B = B; f.T = T; f.Hq = Hq; f.Hkv = Hkv; f.hd = hd; f.scale = scale; f.slots = 1 + p.far.chunks;
+  f.slot_rows = p.sinks;                        // but only those of tiles with far query tiles are in use
+  f.sinks = p.sinks < p.far.tiles * AB_TILE ? p.sinks : p.far.tiles * AB_TILE;
+  f.k_rows = cosT != nullptr ? T : f.sinks;
+  f.v_rows = f.sinks;
+  const long long items = ((long long)B * Hq * T + (long long)B * Hkv * (f.k_rows + f.v_rows)) * (hd / 16), blocks = (items + 255) / 256;
+  const int cb = (int)(blocks < num_sms() * 16 ? blocks : num_sms() * 16);
+  return launch_overlapped(attn_window_finish_kernel, dim3(cb), dim3(256), 0, st, 1, f);
 }

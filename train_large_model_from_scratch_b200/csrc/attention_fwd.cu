@@ -18,7 +18,10 @@
 //              than 2^8, and S of tile j+1 is issued while tile j's softmax runs
 // Shared memory is 80 KB and tensor memory 256 columns (hd 64), so two CTAs share an
 // SM and one CTA's softmax overlaps the other's MMAs. All waits are bounded.
+//
+// WIN, a second instantiation: a sliding window with sinks (see window_plan.h), q, k and v as tensors of their own.
 #include "common.cuh"
+#include "window_plan.h"
 
 namespace tlm {
 
@@ -41,7 +44,18 @@ struct AttnFwdParams {
   int n_dst, dst_rows, dst_heads, dst_head0;
   int hd;                  // head dim of the tensors in memory (= the kernel's HD)
   int head_group;          // heads per group of the heavy-first block order (see heavy_first_decode)
+  int window, sinks;       // WIN: keys a query sees, itself included (at most T), and first keys that stay visible
 };
+
+// WIN: q [.., Hq, hd], k and v [.., Hkv, hd]; else one map over the packed tensor
+template <bool WIN> struct AttnFwdMaps { CUtensorMap qkv; };
+template <> struct AttnFwdMaps<true> { CUtensorMap q, k, v; };
+
+// The first n of 128 positions, as the word with positions 32 w .. 32 w + 31
+__device__ __forceinline__ uint32_t first_bits(int n, int w) {
+  n -= 32 * w;
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
 
 template <int HD>
 struct AttnFwdSmem {
@@ -62,9 +76,9 @@ struct AttnFwdSmem {
 // is used for P and for the final normalisation.
 constexpr float RESCALE_LOG2 = 8.0f;
 
-template <int HD>
+template <int HD, bool WIN = false>
 __global__ void __launch_bounds__(AT_THREADS, HD <= 64 ? 2 : 1)
-attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const AttnFwdParams p) {
+attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams p) {
   using L = AttnFwdSmem<HD>;
   constexpr int KB = L::KB;
   // tensor-memory columns: S (128 fp32), O (HD fp32) and the probabilities as packed bf16 pairs (64 columns),
@@ -95,13 +109,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const AttnFwdParams 
   const int b = bh / p.Hq, h = bh % p.Hq;
   const int kvh = h / (p.Hq / p.Hkv);
   const int q0 = qt * AT_BQ;
-  const int n_kv = qt + 1;                            // causal: KV tiles 0..qt
+  const int first = WIN ? win_first_tile(qt, p.window) : 0;
+  const int n_kv = WIN ? qt - first + 1 + win_sink_tiles(first, p.sinks) : qt + 1;      // causal: KV tiles 0..qt
+  auto kv_row = [&](int j) { return (WIN ? win_kv_tile(j, qt, first) : j) * AT_BKV; };
+  const CUtensorMap *tm_q, *tm_k, *tm_v;
+  int k_head = kvh, v_head = kvh;
+  if constexpr (WIN) { tm_q = &tm.q; tm_k = &tm.k; tm_v = &tm.v; }
+  else { tm_q = tm_k = tm_v = &tm.qkv; k_head += p.Hq; v_head += p.Hq + p.Hkv; }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 13; ++i) mbar_init(bar(i), (i == 8 || i == 10) ? 4 : 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tm_qkv);
+    tma_prefetch_desc(tm_q);
+    if (WIN) { tma_prefetch_desc(tm_k); tma_prefetch_desc(tm_v); }
   }
   if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
   tc_fence_before();
@@ -114,14 +135,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const AttnFwdParams 
     if (lane == 0) {
       mbar_expect_tx(bar(0), L::Q_BYTES);
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) tma_load_4d(sbase + L::OFF_Q + kb * 16384, &tm_qkv, bar(0), kb * 64, h, q0, b);
+      for (int kb = 0; kb < KB; ++kb) tma_load_4d(sbase + L::OFF_Q + kb * 16384, tm_q, bar(0), kb * 64, h, q0, b);
       auto load_k = [&](int j) -> bool {
         const int st = j & 1;
         if (!mbar_wait(bar(11 + st), ((uint32_t)(j >> 1) & 1u) ^ 1u, 11, abort_flag, p.status)) return false;
         mbar_expect_tx(bar(1 + st), L::KV_BYTES);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-          tma_load_4d(sbase + L::OFF_K + st * L::KV_BYTES + kb * 16384, &tm_qkv, bar(1 + st), kb * 64, p.Hq + kvh, j * AT_BKV, b);
+          tma_load_4d(sbase + L::OFF_K + st * L::KV_BYTES + kb * 16384, tm_k, bar(1 + st), kb * 64, k_head, kv_row(j), b);
         return true;
       };
       bool ok = load_k(0);
@@ -132,7 +153,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const AttnFwdParams 
         mbar_expect_tx(bar(3 + st), L::KV_BYTES);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-          tma_load_4d(sbase + L::OFF_V + st * L::KV_BYTES + kb * 16384, &tm_qkv, bar(3 + st), kb * 64, p.Hq + p.Hkv + kvh, j * AT_BKV, b);
+          tma_load_4d(sbase + L::OFF_V + st * L::KV_BYTES + kb * 16384, tm_v, bar(3 + st), kb * 64, v_head, kv_row(j), b);
       }
     }
   } else if (warp == 1) {
@@ -190,7 +211,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const AttnFwdParams 
       const uint32_t par = (uint32_t)j & 1u;
       if (!mbar_wait_warp(bar(7), par, 16, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      const bool diag = (j == qt);
+      const bool diag = !WIN && j == qt;
       // ---- the whole S row (128 fp32) moves to registers in one go; S may then be overwritten by the next
       // tile's Q K^T, which therefore overlaps all of this tile's softmax
       uint32_t sr[AT_BKV];
@@ -200,6 +221,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const AttnFwdParams 
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(10));
+      if constexpr (WIN) {
+        const int t = win_kv_tile(j, qt, first);
+        if (win_partial(qt, t, p.window, p.sinks)) {            // hidden scores become -infinity: probability 0, whatever they were
+          const int last = (qt - t) * AT_BKV + row;             // this row's own position in the tile
+          uint32_t seen[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            seen[w] = first_bits(last + 1, w) & (~first_bits(last + 1 - p.window, w) | first_bits(p.sinks - t * AT_BKV, w));
+#pragma unroll
+          for (int i = 0; i < AT_BKV; ++i)
+            if (!((seen[i >> 5] >> (i & 31)) & 1u)) sr[i] = 0xff800000u;
+        }
+      }
       // ---- row maximum
       float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
       if (!diag) {
@@ -304,17 +338,27 @@ int make_qkv_map(CUtensorMap* map, const void* base, int B, int T, int heads, in
   return make_tmap_bf16(map, base, 4, dims, strides, box);
 }
 
-template <int HD>
-static int launch_fwd(const CUtensorMap& map, const AttnFwdParams& p, cudaStream_t st) {
+template <int HD, bool WIN = false>
+static int launch_fwd(const AttnFwdMaps<WIN>& maps, const AttnFwdParams& p, cudaStream_t st) {
   using L = AttnFwdSmem<HD>;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
   const int grid = ((p.T + AT_BQ - 1) / AT_BQ) * p.B * p.Hq;
-  return launch_overlapped(attn_fwd_kernel<HD>, dim3(grid), dim3(AT_THREADS), L::TOTAL, st, 1, map, p);
+  return launch_overlapped(attn_fwd_kernel<HD, WIN>, dim3(grid), dim3(AT_THREADS), L::TOTAL, st, 1, maps, p);
+}
+
+// The same over any [B, T, heads, hd] tensor; strides (batch, token, head) in elements, multiples of 8
+int make_bthd_map(CUtensorMap* map, const void* base, const long long* strides, int B, int T, int heads, int hd, int box_rows, int box_cols) {
+  if (!aligned16(base)) return -7;
+  for (int i = 0; i < 3; ++i) if (strides[i] <= 0 || strides[i] % 8 != 0 || strides[i] >= (1LL << 39)) return -7;
+  uint64_t dims[4] = {(uint64_t)hd, (uint64_t)heads, (uint64_t)T, (uint64_t)B};
+  uint64_t bytes[3] = {(uint64_t)strides[2] * 2, (uint64_t)strides[1] * 2, (uint64_t)strides[0] * 2};
+  uint32_t box[4] = {(uint32_t)box_cols, 1, (uint32_t)box_rows, 1};
+  return make_tmap_bf16(map, base, 4, dims, bytes, box);
 }
 
 }  // namespace tlm
@@ -326,8 +370,8 @@ static int attn_fwd_impl(const void* qkv, void* o, float* lse, int B, int T, int
   if (hd != 32 && hd != 64 && hd != 128) return -4;
   if (Hq % Hkv != 0) return -5;
   if (n_dst < 0 || n_dst > AT_MAX_DST || (n_dst > 0 && (dst_rows <= 0 || (long long)dst_rows * n_dst < T))) return -6;
-  CUtensorMap map;
-  int e = make_qkv_map(&map, qkv, B, T, Hq + 2 * Hkv, hd, AT_BQ, hd == 32 ? 32 : 64);
+  AttnFwdMaps<false> map;
+  int e = make_qkv_map(&map.qkv, qkv, B, T, Hq + 2 * Hkv, hd, AT_BQ, hd == 32 ? 32 : 64);
   if (e) return e;
   AttnFwdParams p{};
   p.o = (__nv_bfloat16*)o; p.lse = lse; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
@@ -354,4 +398,27 @@ TLM_API int tlm_attn_fwd_scatter(const void* qkv, void* o, float* lse, int B, in
                                  float scale, void* const* o_dst, int n_dst, int dst_rows, int dst_heads,
                                  int dst_head0, cudaStream_t st) {
   return attn_fwd_impl(qkv, o, lse, B, T, Hq, Hkv, hd, scale, o_dst, n_dst, dst_rows, dst_heads, dst_head0, st);
+}
+
+// Causal attention over a sliding window with sinks (window_plan.h) on q [B, T, Hq, hd], k and v [B, T, Hkv, hd]; strides[9]: batch,
+// token and head strides of q, k and v in elements. window <= 0 or above T: no window. o [B, T, Hq, hd], lse [B, Hq, T] contiguous.
+TLM_API int tlm_attn_window_fwd(const void* q, const void* k, const void* v, const long long* strides, void* o, float* lse, int B, int T,
+                                int Hq, int Hkv, int hd, float scale, int window, int sinks, cudaStream_t st) {
+  if (hd != 32 && hd != 64 && hd != 128) return -4;
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return -5;
+  if (B < 0 || T < 0 || T > (1 << 30) || sinks < 0 || (long long)((T + AT_BQ - 1) / AT_BQ) * B * Hq > 0x7fffffffLL) return -6;
+  if (B == 0 || T == 0) return 0;
+  AttnFwdMaps<true> maps;
+  const int cols = hd == 32 ? 32 : 64;
+  int e = make_bthd_map(&maps.q, q, strides, B, T, Hq, hd, AT_BQ, cols);
+  if (!e) e = make_bthd_map(&maps.k, k, strides + 3, B, T, Hkv, hd, AT_BKV, cols);
+  if (!e) e = make_bthd_map(&maps.v, v, strides + 6, B, T, Hkv, hd, AT_BKV, cols);
+  if (e) return e;
+  AttnFwdParams p{};
+  p.o = (__nv_bfloat16*)o; p.lse = lse; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
+  p.scale_log2 = scale * 1.4426950408889634f; p.scale = scale; p.status = status_word(); p.hd = hd;
+  p.window = window > 0 && window < T ? window : T;
+  p.sinks = sinks < T ? sinks : T;
+  p.head_group = attn_head_group("TLM_ATTN_FWD_GROUP", 8LL * T * hd, 64LL << 20, B * Hq);
+  return hd == 128 ? launch_fwd<128, true>(maps, p, st) : hd == 64 ? launch_fwd<64, true>(maps, p, st) : launch_fwd<32, true>(maps, p, st);
 }

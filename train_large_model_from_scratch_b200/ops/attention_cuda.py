@@ -119,3 +119,43 @@ def bwd(do, qkv, o, lse, n_q: int, n_kv: int, causal: bool, rope=None):
         dk = dk.reshape(B, n_kv, rep, T, hd).sum(2)
         dv = dv.reshape(B, n_kv, rep, T, hd).sum(2)
     return torch.cat([dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2)], dim=2).contiguous()
+
+
+def _tiled(t: torch.Tensor) -> torch.Tensor:
+    """`t [B, T, H, hd]` as tiles can be loaded from it: rows contiguous, 16-byte aligned, at strides of whole 16 bytes. Anything
+    else is copied (a broadcast tensor, an odd slice)."""
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in t.stride()[:3])
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int):
+    """Causal attention of `q [B, T, Hq, hd]` over `k`, `v [B, T, Hkv, hd]` (bf16, hd 32 / 64 / 128, strided) where a query sees
+    `window` keys, itself included (0: all), and the first `sinks`. -> o `[B, T, Hq, hd]` bf16, lse `[B, Hq, T]` fp32."""
+    q, k, v = _tiled(q), _tiled(k), _tiled(v)
+    B, T, n_q, hd = q.shape
+    o = torch.empty(B, T, n_q, hd, dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty(B, n_q, T, dtype=torch.float32, device=q.device)
+    native._check(native.lib().tlm_attn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), native._strides(q, k, v), o.data_ptr(),
+                                                   lse.data_ptr(), B, T, n_q, k.shape[2], hd, 1.0 / math.sqrt(hd), min(window, T),
+                                                   min(sinks, T), native._stream()), "attn_window_fwd")
+    return o, lse
+
+
+def window_bwd(do, q, k, v, o, lse, window: int, sinks: int, out, rope=None) -> None:
+    """Gradients of `window_fwd` into `out = (dq, dk, dv)` (bf16, rows contiguous, 16-byte aligned). `rope`: as in `bwd`."""
+    q, k, v = _tiled(q), _tiled(k), _tiled(v)
+    do = do.contiguous()
+    if do.data_ptr() % 16:
+        do = do.clone()
+    B, T, n_q, hd = q.shape
+    n_kv = k.shape[2]
+    f32 = dict(dtype=torch.float32, device=q.device)
+    dq_acc, delta = torch.empty(B, n_q, T, hd, **f32), torch.empty(B, n_q, T, **f32)
+    window, sinks = min(window, T), min(sinks, T)
+    n_part = native.lib().tlm_attn_window_part_floats(B, T, n_kv, hd, window, sinks)
+    part = torch.empty(n_part, **f32) if n_part else None
+    cos, sin = rope if rope is not None else (None, None)
+    native._check(native.lib().tlm_attn_window_bwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), native._strides(q, k, v), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
+        *(t.data_ptr() for t in out), native._strides(*out), dq_acc.data_ptr(), delta.data_ptr(), native._ptr(part), B, T, n_q, n_kv,
+        hd, 1.0 / math.sqrt(hd), native._ptr(cos), native._ptr(sin), window, sinks, native._stream()), "attn_window_bwd")

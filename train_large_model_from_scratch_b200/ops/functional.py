@@ -246,7 +246,7 @@ def qkv_project(h, weight, cos, sin, cs, B: int, T: int, n_q: int, n_kv: int, hd
 
 
 # --------------------------------------------------------------------------- attention
-def _attn_fwd_ref(q, k, v, causal):
+def _attn_fwd_ref(q, k, v, causal, window=0, sinks=0):
     """Returns (out, lse) with fp32 math. q [B,T,Hq,hd], k/v [B,T,Hkv,hd]."""
     B, Tq, Hq, hd = q.shape
     rep = Hq // k.shape[2]
@@ -256,11 +256,32 @@ def _attn_fwd_ref(q, k, v, causal):
     s = qf @ kf.transpose(-1, -2) / math.sqrt(hd)
     if causal:
         mask = torch.ones(Tq, k.shape[1], dtype=torch.bool, device=q.device).triu(1)
+        if window > 0:
+            mask = ~oracle.window_mask(Tq, window, sinks, q.device)
         s = s.masked_fill(mask, float("-inf"))
     lse = torch.logsumexp(s, dim=-1)                              # B,Hq,Tq
     p = torch.exp(s - lse[..., None])
     o = (p @ vf).permute(0, 2, 1, 3)
     return o, lse, p, qf, kf, vf
+
+
+def _attn_bwd_ref(do, q, k, v, o, causal, window=0, sinks=0):
+    """(dq, dk, dv) with fp32 math."""
+    B, T, n_q, hd = q.shape
+    n_kv = k.shape[2]
+    rep = n_q // n_kv
+    _, _, p, qf, kf, vf = _attn_fwd_ref(q, k, v, causal, window, sinks)
+    dof = do.float().permute(0, 2, 1, 3)                       # B,Hq,T,hd
+    of = o.float().permute(0, 2, 1, 3)
+    dv = p.transpose(-1, -2) @ dof
+    dp = dof @ vf.transpose(-1, -2)
+    delta = (dof * of).sum(-1, keepdim=True)
+    ds = p * (dp - delta) / math.sqrt(hd)
+    dq = ds @ kf
+    dk = ds.transpose(-1, -2) @ qf
+    dk = dk.view(B, n_kv, rep, -1, hd).sum(2)
+    dv = dv.view(B, n_kv, rep, -1, hd).sum(2)
+    return [t.permute(0, 2, 1, 3) for t in (dq, dk, dv)]
 
 
 class _Attention(torch.autograd.Function):
@@ -289,26 +310,204 @@ class _Attention(torch.autograd.Function):
         if _use_native(qkv):
             return native.flash_attn_bwd(do.contiguous(), qkv, o, lse, n_q, n_kv, ctx.causal), None, None, None
         q, k, v = qkv[:, :, :n_q], qkv[:, :, n_q:n_q + n_kv], qkv[:, :, n_q + n_kv:]
-        B, T, _, hd = q.shape
-        rep = n_q // n_kv
-        _, _, p, qf, kf, vf = _attn_fwd_ref(q, k, v, ctx.causal)
-        dof = do.float().permute(0, 2, 1, 3)                       # B,Hq,T,hd
-        of = o.float().permute(0, 2, 1, 3)
-        dv = p.transpose(-1, -2) @ dof
-        dp = dof @ vf.transpose(-1, -2)
-        delta = (dof * of).sum(-1, keepdim=True)
-        ds = p * (dp - delta) / math.sqrt(hd)
-        dq = ds @ kf
-        dk = ds.transpose(-1, -2) @ qf
-        dk = dk.view(B, n_kv, rep, -1, hd).sum(2)
-        dv = dv.view(B, n_kv, rep, -1, hd).sum(2)
-        dqkv = torch.cat([dq.permute(0, 2, 1, 3), dk.permute(0, 2, 1, 3), dv.permute(0, 2, 1, 3)], dim=2)
+        dqkv = torch.cat(_attn_bwd_ref(do, q, k, v, o, ctx.causal), dim=2)
         return dqkv.to(qkv.dtype), None, None, None
 
 
-def attention_packed(qkv: torch.Tensor, n_q: int, n_kv: int, causal: bool = True) -> torch.Tensor:
-    """-> `[B, T, Hq, hd]`"""
-    return _Attention.apply(qkv, n_q, n_kv, causal)
+def attention_packed(qkv: torch.Tensor, n_q: int, n_kv: int, causal: bool = True, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """-> `[B, T, Hq, hd]`. `window` > 0: a query sees that many keys, itself included, and besides them the first `sinks` keys of
+    the sequence (see `window_attention`)."""
+    if window == 0 and sinks == 0:
+        return _Attention.apply(qkv, n_q, n_kv, causal)
+    if not causal:
+        raise ValueError("a window needs causal attention")
+    if qkv.dim() != 4 or qkv.shape[2] != n_q + 2 * n_kv:
+        raise ValueError(f"qkv has to be [B, T, {n_q + 2 * n_kv}, hd], not {tuple(qkv.shape)}")
+    _check_window(*_heads_of(qkv, n_q, n_kv), window, sinks)
+    return _WindowPacked.apply(qkv, n_q, n_kv, window, sinks)
+
+
+# --------------------------------------------------------------------------- attention over a sliding window with sinks
+def _heads_of(qkv, n_q, n_kv):
+    return qkv[:, :, :n_q], qkv[:, :, n_q:n_q + n_kv], qkv[:, :, n_q + n_kv:]
+
+
+def _check_device(*tensors) -> None:
+    """CUDA tensors of one call lie on the current device, whose stream the kernels are issued to."""
+    dev = tensors[0].device
+    if any(t.device != dev for t in tensors):
+        raise ValueError("tensors on different devices: " + ", ".join(str(t.device) for t in tensors))
+    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}: "
+                         f"call under torch.cuda.device({dev.index})")
+
+
+def _check_window(q, k, v, window, sinks) -> None:
+    if q.dim() != 4 or k.shape != v.shape or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"q [B, T, Hq, hd] with k and v [B, T, Hkv, hd] expected, not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"the number of query heads ({q.shape[2]}) has to be a multiple of the number of KV heads ({k.shape[2]})")
+    if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
+        raise ValueError(f"window {window}, sinks {sinks}: neither may be negative, and sinks need a window")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"q, k and v of one type expected, not {q.dtype}, {k.dtype}, {v.dtype}")
+    _check_device(q, k, v)
+    if _use_native(q) and q.shape[3] not in (32, 64, 128):
+        raise ValueError(f"head dim {q.shape[3]}: the window kernels have 32, 64 and 128")
+
+
+class _Window(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks):
+        ctx.meta = (window, sinks)
+        if _use_native(q):
+            o, lse = native.window_attn_fwd(q, k, v, window, sinks)
+        else:
+            o, lse, *_ = _attn_fwd_ref(q, k, v, True, window, sinks)
+            o = o.to(q.dtype).contiguous()
+        ctx.save_for_backward(q, k, v, o, lse)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        if _use_native(q):
+            out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+            native.window_attn_bwd(do, q, k, v, o, lse, *ctx.meta, out)
+        else:
+            out = [g.to(q.dtype) for g in _attn_bwd_ref(do, q, k, v, o, True, *ctx.meta)]
+        return *out, None, None
+
+
+class _WindowPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, n_q, n_kv, window, sinks):
+        ctx.meta = (n_q, n_kv, window, sinks)
+        q, k, v = _heads_of(qkv, n_q, n_kv)
+        if _use_native(qkv):
+            o, lse = native.window_attn_fwd(q, k, v, window, sinks)
+        else:
+            o, lse, *_ = _attn_fwd_ref(q, k, v, True, window, sinks)
+            o = o.to(qkv.dtype).contiguous()
+        ctx.save_for_backward(qkv, o, lse)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        qkv, o, lse = ctx.saved_tensors
+        n_q, n_kv, window, sinks = ctx.meta
+        q, k, v = _heads_of(qkv, n_q, n_kv)
+        if _use_native(qkv):
+            dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+            native.window_attn_bwd(do, q, k, v, o, lse, window, sinks, _heads_of(dqkv, n_q, n_kv))
+        else:
+            dqkv = torch.cat(_attn_bwd_ref(do, q, k, v, o, True, window, sinks), dim=2).to(qkv.dtype)
+        return dqkv, None, None, None, None
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """Causal GQA attention of `q [B, T, Hq, hd]` over `k`, `v [B, T, Hkv, hd]` -> `[B, T, Hq, hd]`: key j is visible to query i iff
+    j <= i and (i - j < window or j < sinks); `window` 0: no window. The three may be views of one another's storage or of a
+    packed tensor; rows that are no whole 16-byte pieces apart are copied first. bf16 on the GPU with head dims 32, 64, 128.
+    Inputs have to be finite where a row's 128 neighbours look: a hidden key's weight is exactly zero, but zero times an infinite
+    or NaN value is NaN."""
+    _check_window(q, k, v, window, sinks)
+    return _Window.apply(q, k, v, window, sinks)
+
+
+# --------------------------------------------------------------------------- rotary positions, norms of queries and keys
+def _check_rotary(x, positions, inv_freq) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    if x.dim() != 4:
+        raise ValueError(f"x has to be [B, T, H, hd], not {tuple(x.shape)}")
+    B, T, _, hd = x.shape
+    if hd % 2 or not 2 <= hd <= 256:
+        raise ValueError(f"head dim {hd}: an even one up to 256 expected")
+    if positions.dtype != torch.int64 or tuple(positions.shape) not in ((T,), (1, T), (B, T)):
+        raise ValueError(f"positions have to be int64 [{T}] or [{B}, {T}], not {positions.dtype} {tuple(positions.shape)}")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 1 <= inv_freq.numel() <= hd // 2:
+        raise ValueError(f"inv_freq has to be float64 with 1 to {hd // 2} frequencies, not {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    _check_device(x, positions, inv_freq)
+    if positions.dim() == 2 and positions.shape[0] == 1:
+        positions = positions[0]
+    if x.stride(3) != 1 and x.shape[3] > 1:
+        x = x.contiguous()
+    return x, positions.contiguous(), inv_freq.contiguous()
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, interleaved, scale):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.meta = (interleaved, scale)
+        return _Rotary.turn(x, positions, inv_freq, interleaved, scale, False)
+
+    @staticmethod
+    def turn(x, positions, inv_freq, interleaved, scale, inverse):
+        if _use_native(x):
+            return native.qk_rotary(x, positions, inv_freq, interleaved=interleaved, scale=scale, inverse=inverse)
+        return oracle.rotary(x, positions, inv_freq, interleaved, scale, inverse).to(x.dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _Rotary.turn(dy.contiguous(), *ctx.saved_tensors, *ctx.meta, True), None, None, None, None
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
+    """Every head of `x [B, T, H, hd]` turned by its token's position: `positions` int64 `[T]` or `[B, T]` (any values), `inv_freq`
+    and `scale` from `oracle.rotary_frequencies`. The first `2 * len(inv_freq)` elements of a head turn, in pairs
+    (i, i + len(inv_freq)) or, `interleaved`, (2 i, 2 i + 1); the rest passes. A new tensor; `x` may be a view (rows contiguous)."""
+    return _Rotary.apply(*_check_rotary(x, positions, inv_freq), bool(interleaved), float(scale))
+
+
+class _QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, n_q, q_weight, k_weight, positions, inv_freq, eps, interleaved, scale):
+        ctx.save_for_backward(x, positions, inv_freq)
+        ctx.weights, ctx.meta = (q_weight, k_weight), (n_q, eps, interleaved, scale)
+        return _qk_norm_fwd(x, ctx.weights, positions, inv_freq, *ctx.meta)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _qk_norm_bwd(dy.contiguous(), *ctx.saved_tensors, ctx.weights, *ctx.meta), *[None] * 8
+
+
+def _qk_norm_fwd(x, weights, positions, inv_freq, n_q, eps, interleaved, scale):
+    if _use_native(x):
+        return native.qk_rotary(x, positions, inv_freq, weights, n_q, eps, interleaved, scale)
+    xf = x.float()
+    hat = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
+    u = torch.cat([hat[:, :, :n_q] * weights[0].float(), hat[:, :, n_q:] * weights[1].float()], dim=2)
+    return oracle.rotary(u, positions, inv_freq, interleaved, scale).to(x.dtype)
+
+
+def _qk_norm_bwd(dy, x, positions, inv_freq, weights, n_q, eps, interleaved, scale, out=None):
+    grads = [_main_grad(w) for w in weights]
+    if _use_native(x):
+        return native.qk_norm_rotary_bwd(dy, x, positions, inv_freq, weights, grads, n_q, eps, interleaved, scale, out)
+    xf = x.float()
+    rstd = torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
+    hat = xf * rstd
+    du = oracle.rotary(dy, positions, inv_freq, interleaved, scale, inverse=True)
+    g = torch.empty_like(du)
+    for w, mg, heads in zip(weights, grads, (slice(0, n_q), slice(n_q, None))):
+        mg.add_((du[:, :, heads] * hat[:, :, heads]).sum((0, 1, 2)))
+        g[:, :, heads] = du[:, :, heads] * w.float()
+    dx = (rstd * (g - hat * (g * hat).mean(-1, keepdim=True))).to(x.dtype)
+    return dx if out is None else out.copy_(dx)
+
+
+def qk_norm_rotary(x: torch.Tensor, n_q: int, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                   inv_freq: torch.Tensor, eps: float = 1e-6, interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
+    """`rotary` behind an RMS norm of every head of `x [B, T, H, hd]`: heads below `n_q` are scaled by `q_weight [hd]`, the others by
+    `k_weight`. The weights' gradients are added to their `main_grad`, like all parameters'."""
+    x, positions, inv_freq = _check_rotary(x, positions, inv_freq)
+    if not 0 <= n_q <= x.shape[2]:
+        raise ValueError(f"n_q {n_q} of {x.shape[2]} heads")
+    for w in (q_weight, k_weight):
+        if tuple(w.shape) != (x.shape[3],) or w.dtype != x.dtype or not w.is_contiguous():
+            raise ValueError(f"weights have to be contiguous {x.dtype} [{x.shape[3]}], not {w.dtype} {tuple(w.shape)}")
+    _check_device(x, q_weight, k_weight)
+    return _QkNormRotary.apply(x, n_q, q_weight, k_weight, positions, inv_freq, float(eps), bool(interleaved), float(scale))
 
 
 # --------------------------------------------------------------------------- SwiGLU

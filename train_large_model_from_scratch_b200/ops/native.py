@@ -83,6 +83,12 @@ _SIGS = {
     "tlm_attn_fwd_scatter": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _I, _I, _I, _I, _P]),
     "tlm_attn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P]),
     "tlm_attn_bwd_scatter": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "tlm_attn_window_fwd": (_I, [_P] * 6 + [_I] * 5 + [_F, _I, _I, _P]),
+    "tlm_attn_window_part_floats": (_LL, [_I] * 6),
+    "tlm_attn_window_bwd": (_I, [_P] * 14 + [_I] * 5 + [_F, _P, _P, _I, _I, _P]),
+    "tlm_qk_rotary": (_I, [_P] * 5 + [_LL, _P, _I, _P, _P] + [_I] * 5 + [_F, _F, _I, _I, _P]),
+    "tlm_qk_norm_work_floats": (_I, [_I]),
+    "tlm_qk_norm_rotary_bwd": (_I, [_P] * 7 + [_LL, _P, _I] + [_P] * 5 + [_I] * 5 + [_F, _F, _I, _P]),
     "tlm_peer_barrier": (_I, [_P, _I, _I, _I, _P]),
     "tlm_wait_flag": (_I, [_P, _I, _c.c_ulonglong, _P]),
     "tlm_reduce_scatter_blocks": (_I, []),
@@ -424,6 +430,40 @@ def rope_qk(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot: int,
     return qkv
 
 
+def _strides(*tensors: torch.Tensor):
+    """Batch, token and head strides of `[B, T, H, hd]` tensors, in elements."""
+    flat = [s for t in tensors for s in t.stride()[:3]]
+    return (ctypes.c_longlong * len(flat))(*flat)
+
+
+def qk_rotary(x, positions, inv_freq, weights=None, n_q: int = 0, eps: float = 0.0, interleaved: bool = False, scale: float = 1.0,
+              inverse: bool = False) -> torch.Tensor:
+    """`x [B, T, H, hd]` bf16 (rows contiguous) rotated by `positions` (int64, `[T]` or `[B, T]`) and `inv_freq` (float64), with
+    `weights = (q, k)` behind an RMS norm of every head (`csrc/qk_rotary.cu`). `inverse`: the transposed rotation, without norm."""
+    B, T, H, hd = x.shape
+    y = torch.empty(B, T, H, hd, dtype=torch.bfloat16, device=x.device)
+    wq, wk = weights if weights is not None else (None, None)
+    _check(lib().tlm_qk_rotary(x.data_ptr(), _strides(x), y.data_ptr(), _strides(y), positions.data_ptr(),
+                               T if positions.dim() > 1 else 0, inv_freq.data_ptr(), inv_freq.numel(), _ptr(wq), _ptr(wk), B, T, H,
+                               n_q, hd, eps, scale, int(interleaved), int(inverse), _stream()), "qk_rotary")
+    return y
+
+
+def qk_norm_rotary_bwd(dy, x, positions, inv_freq, weights, grads, n_q: int, eps: float, interleaved: bool, scale: float, out=None):
+    """Gradient of `qk_rotary` with norm; the weights' gradients are added to `grads = (q, k)` (fp32). `out`: where it goes, may be
+    `dy` itself."""
+    B, T, H, hd = x.shape
+    if out is None:
+        out = torch.empty(B, T, H, hd, dtype=torch.bfloat16, device=x.device)
+    work = torch.empty(lib().tlm_qk_norm_work_floats(hd), dtype=torch.float32, device=x.device)
+    _check(lib().tlm_qk_norm_rotary_bwd(x.data_ptr(), _strides(x), dy.data_ptr(), _strides(dy), out.data_ptr(), _strides(out),
+                                        positions.data_ptr(), T if positions.dim() > 1 else 0, inv_freq.data_ptr(), inv_freq.numel(),
+                                        weights[0].data_ptr(), weights[1].data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(),
+                                        work.data_ptr(), B, T, H, n_q, hd, eps, scale, int(interleaved), _stream()),
+           "qk_norm_rotary_bwd")
+    return out
+
+
 def swiglu_fwd(gu: torch.Tensor, valid_rows: torch.Tensor | None = None) -> torch.Tensor:
     """`valid_rows` (optional 1-element int64 device tensor): only that many leading rows are computed."""
     gu = gu.contiguous()
@@ -526,6 +566,16 @@ def flash_attn_bwd(do, qkv, o, lse, n_q: int, n_kv: int, causal: bool, rope=None
     the gradient of the un-rotated q and k (done in fp32 as the gradients leave the kernels)."""
     from . import attention_cuda
     return attention_cuda.bwd(do, qkv, o, lse, n_q, n_kv, causal, rope)
+
+
+def window_attn_fwd(q, k, v, window: int, sinks: int):
+    from . import attention_cuda
+    return attention_cuda.window_fwd(q, k, v, window, sinks)
+
+
+def window_attn_bwd(do, q, k, v, o, lse, window: int, sinks: int, out, rope=None) -> None:
+    from . import attention_cuda
+    attention_cuda.window_bwd(do, q, k, v, o, lse, window, sinks, out, rope)
 
 
 # --------------------------------------------------------------------------- grouped GEMMs (MoE experts)

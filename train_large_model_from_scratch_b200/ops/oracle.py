@@ -65,6 +65,65 @@ def rope_bwd(dy: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Te
     return df * c + rotate_half_t(df * s)
 
 
+ROPE_SCALINGS = ("none", "linear", "ntk", "yarn")
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       original_length: int = 4096, device=None) -> tuple[torch.Tensor, float]:
+    """Frequencies (float64 `[rotary_dim / 2]`, radians per position) and the factor on cos and sin, for `rotary`.
+
+    scaling "linear": positions are divided by `factor`. "ntk": theta grows so that the slowest pair turns `factor` times slower.
+    "yarn": pairs that turn more than 32 times within `original_length` stay, those below one turn are divided by `factor`, with
+    a linear ramp over the pair index between; cos and sin are multiplied by 0.1 ln(factor) + 1.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, not {rotary_dim}")
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"unknown scaling {scaling!r}: one of {ROPE_SCALINGS}")
+    if theta <= 1.0 or factor < 1.0 or original_length < 1:
+        raise ValueError("theta has to be above 1, factor at least 1, original_length positive")
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("scaling 'ntk' needs a rotary_dim of at least 4")
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+    freq = theta ** (-2.0 * i / rotary_dim)
+    if scaling == "linear":
+        freq = freq / factor
+    if scaling != "yarn":
+        return freq, 1.0
+
+    def pair_of(turns: float) -> float:           # index of the pair that turns so often within original_length
+        return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    low, high = max(0, math.floor(pair_of(32.0))), min(rotary_dim // 2 - 1, math.ceil(pair_of(1.0)))
+    ramp = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+    return freq * (1.0 - ramp) + freq / factor * ramp, 0.1 * math.log(factor) + 1.0
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0,
+           inverse: bool = False) -> torch.Tensor:
+    """x: `[B, T, H, hd]`; positions `[T]` or `[B, T]`; the first 2 * len(inv_freq) of a head turn, pairs (i, i + len) or (2i, 2i + 1).
+    `inverse`: the transposed map (backward). Angles in 64 bits, the rest in 32."""
+    r = 2 * inv_freq.numel()
+    angle = positions.double()[..., None] * inv_freq.double()
+    cos, sin = (scale * f(angle).float()[..., None, :] for f in (torch.cos, torch.sin))
+    if inverse:
+        sin = -sin
+    xf = x.float()
+    a, b = (xf[..., 0:r:2], xf[..., 1:r:2]) if interleaved else (xf[..., :r // 2], xf[..., r // 2:r])
+    ya, yb = a * cos - b * sin, b * cos + a * sin
+    y = torch.stack([ya, yb], dim=-1).flatten(-2) if interleaved else torch.cat([ya, yb], dim=-1)
+    return torch.cat([y, xf[..., r:]], dim=-1)
+
+
+def window_mask(T: int, window: int, sinks: int, device=None) -> torch.Tensor:
+    """`[T, T]` bool: does query row see key column? `window` 0: every key up to the query."""
+    i, j = torch.arange(T, device=device)[:, None], torch.arange(T, device=device)
+    seen = j <= i
+    return seen if window <= 0 else seen & ((i - j < window) | (j < sinks))
+
+
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True,
               q_offset: int = 0) -> torch.Tensor:
     """q: [B, Tq, Hq, hd], k/v: [B, Tk, Hkv, hd] -> [B, Tq, Hq, hd].
