@@ -212,6 +212,23 @@ def test_same_bits_again_and_in_a_graph():
             assert ((dq.float() - want[s][1].float()).abs() <= 2 * H * dq.float().abs() + 1e-5 * dq.abs().max()).all()
 
 
+def test_first_call_of_a_thread():
+    """Tensor maps are made through the driver, which a thread's first CUDA call has to have prepared."""
+    import threading
+    got = []
+    x = torch.zeros(1, 77, 4, 64, device="cuda", dtype=torch.bfloat16)
+
+    def call():
+        from train_large_model_from_scratch_b200.ops import native
+        got.append(native.window_attn_fwd(x[:, :, :2], x[:, :, 2:3], x[:, :, 3:], 11, 1)[0])
+
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1 and (got[0] == 0).all()
+
+
 def test_gradients_against_differences():
     """The gradient of sum(o * do) along a random direction, against central differences of the definition."""
     from train_large_model_from_scratch_b200.ops import oracle

@@ -31,9 +31,33 @@ struct QrParams {
 };
 
 // Sixteen elements of a row are one lane's: eight pairs (8 l + i), the rotated ones first, then what passes through, paired up in
-// the same way. v[va(i)], v[vb(i)] are pair i. VEC: two 16-byte pieces; else element by element (odd widths, strides, addresses).
-template <bool INTER> __device__ __forceinline__ constexpr int va(int i) { return INTER ? 2 * i : i; }
-template <bool INTER> __device__ __forceinline__ constexpr int vb(int i) { return INTER ? 2 * i + 1 : i + 8; }
+// the same way. In registers the first and second elements of the pairs are four packed fp32 pairs each (a, b): two lanes of
+// arithmetic an issue slot. Issue is what bounded these kernels: B 8, T 4096, 16 + 8 heads of 64 took 56 us forward and 73 backward
+// with scalar arithmetic, weights selected in registers and addresses worked out row by row (1146 instructions a token and warp).
+struct Packed { uint32_t w[8]; };                       // as they lie in memory: half layout 4 words of a, 4 of b; interleaved (a, b) each
+struct Pairs { float2 a[4], b[4]; };
+
+template <bool INTER>
+__device__ __forceinline__ Pairs unpack(const Packed& r) {
+  Pairs v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 x = unpack_bf16(r.w[INTER ? 2 * j : j]), y = unpack_bf16(r.w[INTER ? 2 * j + 1 : j + 4]);
+    v.a[j] = INTER ? make_float2(x.x, y.x) : x;
+    v.b[j] = INTER ? make_float2(x.y, y.y) : y;
+  }
+  return v;
+}
+template <bool INTER>
+__device__ __forceinline__ Packed pack(const Pairs& v) {
+  Packed r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    r.w[INTER ? 2 * j : j] = INTER ? pack_bf16(v.a[j].x, v.b[j].x) : pack_bf16(v.a[j].x, v.a[j].y);
+    r.w[INTER ? 2 * j + 1 : j + 4] = INTER ? pack_bf16(v.a[j].y, v.b[j].y) : pack_bf16(v.b[j].x, v.b[j].y);
+  }
+  return r;
+}
 
 template <bool INTER>
 __device__ __forceinline__ void pair_at(int pair, int hd, int n_freq, int& a, int& b) {
@@ -42,79 +66,75 @@ __device__ __forceinline__ void pair_at(int pair, int hd, int n_freq, int& a, in
   else { a = n_freq + pair; b = a + (hd - 2 * n_freq) / 2; }      // 2 n_freq + (pair - n_freq)
 }
 
+// Where a lane's elements lie. VEC: two 16-byte pieces at a and b; else element by element (odd widths, strides, addresses).
 template <bool INTER, bool VEC>
-__device__ __forceinline__ void load_row(const __nv_bfloat16* row, int l, int hd, int n_freq, bool ok, float* v) {
-  if (VEC) {
-    int a, b;
+struct RowMap {
+  int a, b, l, hd, n_freq;
+  bool any;                                             // this lane has elements
+  __device__ RowMap(int lane_of_row, int hd_, int n_freq_) : l(lane_of_row), hd(hd_), n_freq(n_freq_) {
     pair_at<INTER>(8 * l, hd, n_freq, a, b);
     if (INTER) b = a + 8;
-    ok = ok && 16 * l < hd;
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    const uint4 lo = ok ? *reinterpret_cast<const uint4*>(row + a) : z, hi = ok ? *reinterpret_cast<const uint4*>(row + b) : z;
-    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    any = 16 * l < hd;
+  }
+  __device__ __forceinline__ Packed load(const __nv_bfloat16* row, bool ok) const {
+    Packed r;
+    if (VEC) {
+      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+      if (ok && any) { lo = *reinterpret_cast<const uint4*>(row + a); hi = *reinterpret_cast<const uint4*>(row + b); }
+      r.w[0] = lo.x; r.w[1] = lo.y; r.w[2] = lo.z; r.w[3] = lo.w; r.w[4] = hi.x; r.w[5] = hi.y; r.w[6] = hi.z; r.w[7] = hi.w;
+    } else {
+      unsigned short e[16];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) { const float2 f = unpack_bf16(w[k]); v[2 * k] = f.x; v[2 * k + 1] = f.y; }
-  } else {
+      for (int i = 0; i < 8; ++i) {
+        int x, y;
+        pair_at<INTER>(8 * l + i, hd, n_freq, x, y);
+        const bool in = ok && 2 * (8 * l + i) < hd;
+        e[INTER ? 2 * i : i] = in ? reinterpret_cast<const unsigned short*>(row)[x] : 0;
+        e[INTER ? 2 * i + 1 : i + 8] = in ? reinterpret_cast<const unsigned short*>(row)[y] : 0;
+      }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      int a, b;
-      pair_at<INTER>(8 * l + i, hd, n_freq, a, b);
-      const bool in = ok && 2 * (8 * l + i) < hd;
-      v[va<INTER>(i)] = in ? __bfloat162float(row[a]) : 0.f;
-      v[vb<INTER>(i)] = in ? __bfloat162float(row[b]) : 0.f;
+      for (int k = 0; k < 8; ++k) r.w[k] = e[2 * k] | ((uint32_t)e[2 * k + 1] << 16);
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* row, const Packed& r) const {
+    if (VEC) {
+      if (!any) return;
+      *reinterpret_cast<uint4*>(row + a) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+      *reinterpret_cast<uint4*>(row + b) = make_uint4(r.w[4], r.w[5], r.w[6], r.w[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (2 * (8 * l + i) >= hd) continue;
+        int x, y;
+        pair_at<INTER>(8 * l + i, hd, n_freq, x, y);
+        const int k = INTER ? 2 * i : i, m = INTER ? 2 * i + 1 : i + 8;
+        reinterpret_cast<unsigned short*>(row)[x] = (unsigned short)(r.w[k >> 1] >> (16 * (k & 1)));
+        reinterpret_cast<unsigned short*>(row)[y] = (unsigned short)(r.w[m >> 1] >> (16 * (m & 1)));
+      }
     }
   }
-}
+};
 
-template <bool INTER, bool VEC>
-__device__ __forceinline__ void store_row(__nv_bfloat16* row, int l, int hd, int n_freq, const float* v) {
-  if (VEC) {
-    if (16 * l >= hd) return;
-    int a, b;
-    pair_at<INTER>(8 * l, hd, n_freq, a, b);
-    if (INTER) b = a + 8;
-    *reinterpret_cast<uint4*>(row + a) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    *reinterpret_cast<uint4*>(row + b) = make_uint4(pack_bf16(v[8], v[9]), pack_bf16(v[10], v[11]), pack_bf16(v[12], v[13]), pack_bf16(v[14], v[15]));
-  } else {
+// Eight floats of shared memory that belong to a lane, as packed pairs
+__device__ __forceinline__ void four_pairs(const float* s, float2* out) {
+  const float4 x = reinterpret_cast<const float4*>(s)[0], y = reinterpret_cast<const float4*>(s)[1];
+  out[0] = make_float2(x.x, x.y); out[1] = make_float2(x.z, x.w);
+  out[2] = make_float2(y.x, y.y); out[3] = make_float2(y.z, y.w);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ void scale_by(Pairs& v, float s) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (2 * (8 * l + i) >= hd) continue;
-      int a, b;
-      pair_at<INTER>(8 * l + i, hd, n_freq, a, b);
-      row[a] = __float2bfloat16(v[va<INTER>(i)]);
-      row[b] = __float2bfloat16(v[vb<INTER>(i)]);
-    }
-  }
+  for (int j = 0; j < 4; ++j) { v.a[j] = fmul2(v.a[j], both(s)); v.b[j] = fmul2(v.b[j], both(s)); }
 }
-
-// m cos and m sin of this lane's eight pairs. The product of position and frequency keeps 64 bits until whole turns are taken off:
-// at position 2^20 a 32-bit product is off by 0.06. Pairs that pass through turn by nothing.
-__device__ __forceinline__ void angles(const QrParams& p, double pos, int l, float* cs, float* sn) {
+// sum of x * y over a lane's sixteen
+__device__ __forceinline__ float dot16(const Pairs& x, const Pairs& y) {
+  float2 s = fmul2(x.a[0], y.a[0]), t = fmul2(x.b[0], y.b[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int pair = 8 * l + i;
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-    if (pair < p.n_freq) {
-      const double turns = pos * (p.inv_freq[pair] * 0.15915494309189533577);      // 1 / (2 pi)
-      float s, c;
-      sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-      cs[i] = p.m * c;
-      sn[i] = p.m * p.sign * s;
-    }
-  }
+  for (int j = 1; j < 4; ++j) { s = ffma2(x.a[j], y.a[j], s); t = ffma2(x.b[j], y.b[j], t); }
+  s = fadd2(s, t);
+  return s.x + s.y;
 }
-
-template <bool INTER>
-__device__ __forceinline__ void rotate(float* v, const float* cs, const float* sn) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = v[va<INTER>(i)], b = v[vb<INTER>(i)];
-    v[va<INTER>(i)] = a * cs[i] - b * sn[i];
-    v[vb<INTER>(i)] = b * cs[i] + a * sn[i];
-  }
-}
-
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v) {
 #pragma unroll
@@ -122,143 +142,256 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// LPR lanes share a row. A warp's 32 / LPR row slots take one token's heads, or those of several tokens where a token has fewer
-// heads: a lane computes its angles once for all heads of its token.
+// Where a lane stands: LPR lanes share a row; a warp's 32 / LPR row slots take one token's heads, or those of several tokens where a
+// token has fewer heads.
+template <int LPR>
+struct QrLane {
+  int lane, warp, l, hps, tpw, h0, tslot;
+  __device__ explicit QrLane(const QrParams& p)
+      : lane(threadIdx.x & 31), warp(threadIdx.x >> 5), l(lane % LPR), hps(1 << p.hps_log), tpw((32 / LPR) >> p.hps_log),
+        h0((lane / LPR) & (hps - 1)), tslot((lane / LPR) >> p.hps_log) {}
+};
+
+// m cos and m sin of a warp's tokens, worked out once for all their heads: [token of the warp][a row's LPR * 8 pairs], (1, 0) for what
+// passes through. The product of position and frequency keeps 64 bits until whole turns are taken off: at position 2^20 a 32-bit
+// product is off by 0.06 radians.
+template <int LPR>
+struct QrAngles {
+  float cos[256], sin[256];                             // 32 / LPR tokens at most
+
+  __device__ void clear(int lane) {
+    for (int k = lane; k < 256; k += 32) { cos[k] = 1.f; sin[k] = 0.f; }
+  }
+  // `pos`: the position of the lane's own token
+  __device__ __forceinline__ void set(const QrParams& p, const QrLane<LPR>& me, double pos) {
+    __syncwarp();                                       // the last tokens' have been read
+    for (int ts = 0; ts < me.tpw; ++ts) {
+      const double at = __shfl_sync(0xffffffffu, pos, (ts << p.hps_log) * LPR);
+      for (int pair = me.lane; pair < p.n_freq; pair += 32) {
+        const double turns = at * (p.inv_freq[pair] * 0.15915494309189533577);      // 1 / (2 pi)
+        float s, c;
+        sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+        cos[ts * LPR * 8 + pair] = p.m * c;
+        sin[ts * LPR * 8 + pair] = p.m * p.sign * s;
+      }
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void rotate(Pairs& v, const QrLane<LPR>& me) const {
+    const int at = (me.tslot * LPR + me.l) * 8;
+    float2 c[4], s[4];
+    four_pairs(cos + at, c);
+    four_pairs(sin + at, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = v.a[j], b = v.b[j], n = fmul2(s[j], both(-1.f));
+      v.a[j] = ffma2(a, c[j], fmul2(b, n));
+      v.b[j] = ffma2(b, c[j], fmul2(a, s[j]));
+    }
+  }
+};
+
+// The two weights in 32 bits, in the lanes' order: [of q, of others][a, b][a row's LPR * 8 pairs]
+template <int LPR, bool INTER, bool VEC>
+struct QrWeights {
+  float w[2][2][LPR * 8];
+
+  __device__ void fill(const QrParams& p) {
+    for (int i = threadIdx.x; i < 2 * LPR * 8; i += QR_THREADS) {
+      const int which = i / (LPR * 8), pair = i % (LPR * 8);
+      int a, b;
+      pair_at<INTER>(pair, p.hd, p.n_freq, a, b);
+      const bool in = 2 * pair < p.hd;
+      w[which][0][pair] = in ? __bfloat162float(p.w[which][a]) : 0.f;
+      w[which][1][pair] = in ? __bfloat162float(p.w[which][b]) : 0.f;
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ void times(Pairs& v, int which, int l) const {
+    float2 x[4];
+    four_pairs(w[which][0] + l * 8, x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.a[j] = fmul2(v.a[j], x[j]);
+    four_pairs(w[which][1] + l * 8, x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.b[j] = fmul2(v.b[j], x[j]);
+  }
+};
+
+// The lane's token: batch entry, place, and whether there is one
+struct QrToken {
+  int b, t;
+  bool in;
+  __device__ __forceinline__ QrToken(const QrParams& p, long long tok) {
+    in = tok < p.tokens;
+    b = in ? (int)tok / p.T : 0;
+    t = in ? (int)tok - b * p.T : 0;
+  }
+  __device__ __forceinline__ __nv_bfloat16* in_tensor(const QrTensor& x, int h) const { return x.p + b * x.sb + t * x.st + h * x.sh; }
+  __device__ __forceinline__ double position(const QrParams& p) const { return in ? (double)p.pos[b * p.pos_sb + t] : 0.; }
+};
+
+// One row is worked on while the next is on its way, the next token's first one included, and its position. (Four rows requested at
+// once, each processed from registers, needed 80 registers and 130 bytes of spills.)
 template <int LPR, bool INTER, bool VEC, bool NORM>
-__global__ void __launch_bounds__(QR_THREADS)
+__global__ void __launch_bounds__(QR_THREADS, VEC ? 4 : 2)
 qk_rotary_fwd_kernel(const QrParams p) {
   griddep_wait();
   griddep_launch();
-  const int lane = threadIdx.x & 31, l = lane % LPR, slot = lane / LPR;
-  const int hps = 1 << p.hps_log, tpw = (32 / LPR) >> p.hps_log;
-  const int h0 = slot & (hps - 1), tslot = slot >> p.hps_log;
-  const int step = gridDim.x * (QR_THREADS / 32) * tpw;
-  float wq[NORM ? 16 : 1], wk[NORM ? 16 : 1];
-  if (NORM) {
-    load_row<INTER, VEC>(p.w[0], l, p.hd, p.n_freq, true, wq);
-    load_row<INTER, VEC>(p.w[1], l, p.hd, p.n_freq, true, wk);
-  }
-  for (long long tok0 = (long long)(blockIdx.x * (QR_THREADS / 32) + (threadIdx.x >> 5)) * tpw; tok0 < p.tokens; tok0 += step) {
-    const int tok = (int)tok0 + tslot;
-    const bool in = tok < p.tokens;
-    const int b = in ? tok / p.T : 0, t = in ? tok - b * p.T : 0;
-    float cs[8], sn[8];
-    angles(p, (double)p.pos[b * p.pos_sb + t], l, cs, sn);
-    const __nv_bfloat16* x = p.in.p + b * p.in.sb + t * p.in.st;
-    __nv_bfloat16* y = p.out.p + b * p.out.sb + t * p.out.st;
-    for (int hb = 0; hb < p.H; hb += hps) {
-      const int h = hb + h0;
-      const bool ok = in && h < p.H;
-      float v[16];
-      load_row<INTER, VEC>(x + h * p.in.sh, l, p.hd, p.n_freq, ok, v);
-      if (NORM) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
-        const float rstd = rsqrtf(row_sum<LPR>(ss) / (float)p.hd + p.eps);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= rstd * (h < p.n_q ? wq[i] : wk[i]);
+  __shared__ __align__(16) QrAngles<LPR> turn_all[QR_THREADS / 32];
+  __shared__ __align__(16) QrWeights<NORM ? LPR : 1, INTER, VEC> weights;
+  const QrLane<LPR> me(p);
+  const RowMap<INTER, VEC> map(me.l, p.hd, p.n_freq);
+  QrAngles<LPR>& turn = turn_all[me.warp];
+  turn.clear(me.lane);
+  if constexpr (NORM) weights.fill(p);
+  const float inv_hd = 1.f / (float)p.hd;
+  const long long ahead = (long long)p.in.sh * me.hps;
+  const int step = gridDim.x * (QR_THREADS / 32) * me.tpw;
+  long long tok0 = (long long)(blockIdx.x * (QR_THREADS / 32) + me.warp) * me.tpw;
+  QrToken now(p, tok0 + me.tslot);
+  const __nv_bfloat16* x = now.in_tensor(p.in, me.h0);
+  Packed raw = map.load(x, now.in && me.h0 < p.H);
+  double pos = now.position(p);
+  for (; tok0 < p.tokens; tok0 += step) {
+    const QrToken next(p, tok0 + step + me.tslot);
+    const __nv_bfloat16* x_next = next.in_tensor(p.in, me.h0);
+    __nv_bfloat16* y = now.in_tensor(p.out, me.h0);
+    turn.set(p, me, pos);
+    pos = next.position(p);
+#pragma unroll 1
+    for (int h = me.h0; h - me.h0 < p.H; h += me.hps) {
+      Pairs v = unpack<INTER>(raw);
+      x += ahead;
+      const bool more = h - me.h0 + me.hps < p.H;       // of the whole warp
+      raw = map.load(more ? x : x_next, more ? now.in && h + me.hps < p.H : next.in && me.h0 < p.H);
+      if constexpr (NORM) {
+        const float rstd = rsqrtf(row_sum<LPR>(dot16(v, v)) * inv_hd + p.eps);
+        weights.times(v, h < p.n_q ? 0 : 1, me.l);
+        scale_by(v, rstd);
       }
-      rotate<INTER>(v, cs, sn);
-      if (ok) store_row<INTER, VEC>(y + h * p.out.sh, l, p.hd, p.n_freq, v);
+      turn.rotate(v, me);
+      if (now.in && h < p.H) map.store(y, pack<INTER>(v));
+      y += p.out.sh * me.hps;
     }
+    now = next;
+    x = x_next;
   }
 }
 
 // Every block leaves its sums for the weights in `part`; qk_norm_dw_kernel adds them up in a fixed order.
 template <int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(QR_THREADS)
+__global__ void __launch_bounds__(QR_THREADS, VEC ? 2 : 1)
 qk_norm_rotary_bwd_kernel(const QrParams p) {
   griddep_wait();
   griddep_launch();
+  __shared__ __align__(16) QrAngles<LPR> turn_all[QR_THREADS / 32];
+  __shared__ __align__(16) QrWeights<LPR, INTER, VEC> weights;
   __shared__ float sums[QR_THREADS / 32][2][LPR * 16];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LPR, slot = lane / LPR;
-  const int hps = 1 << p.hps_log, tpw = (32 / LPR) >> p.hps_log;
-  const int h0 = slot & (hps - 1), tslot = slot >> p.hps_log;
-  const int step = gridDim.x * (QR_THREADS / 32) * tpw;
-  float wq[16], wk[16], dq[16], dk[16];
-  load_row<INTER, VEC>(p.w[0], l, p.hd, p.n_freq, true, wq);
-  load_row<INTER, VEC>(p.w[1], l, p.hd, p.n_freq, true, wk);
+  const QrLane<LPR> me(p);
+  const RowMap<INTER, VEC> map(me.l, p.hd, p.n_freq);
+  QrAngles<LPR>& turn = turn_all[me.warp];
+  turn.clear(me.lane);
+  weights.fill(p);
+  const float inv_hd = 1.f / (float)p.hd;
+  Pairs dq, dk;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) dq[i] = dk[i] = 0.f;
-  for (long long tok0 = (long long)(blockIdx.x * (QR_THREADS / 32) + warp) * tpw; tok0 < p.tokens; tok0 += step) {
-    const int tok = (int)tok0 + tslot;
-    const bool in = tok < p.tokens;
-    const int b = in ? tok / p.T : 0, t = in ? tok - b * p.T : 0;
-    float cs[8], sn[8];
-    angles(p, (double)p.pos[b * p.pos_sb + t], l, cs, sn);
-    const __nv_bfloat16* x = p.x.p + b * p.x.sb + t * p.x.st;
-    const __nv_bfloat16* dy = p.in.p + b * p.in.sb + t * p.in.st;
-    __nv_bfloat16* dx = p.out.p + b * p.out.sb + t * p.out.st;
-    for (int hb = 0; hb < p.H; hb += hps) {
-      const int h = hb + h0;
-      const bool ok = in && h < p.H, is_q = h < p.n_q;
-      float v[16], g[16];
-      load_row<INTER, VEC>(x + h * p.x.sh, l, p.hd, p.n_freq, ok, v);
-      load_row<INTER, VEC>(dy + h * p.in.sh, l, p.hd, p.n_freq, ok, g);
-      float ss = 0.f;
+  for (int j = 0; j < 4; ++j) dq.a[j] = dq.b[j] = dk.a[j] = dk.b[j] = make_float2(0.f, 0.f);
+  const int step = gridDim.x * (QR_THREADS / 32) * me.tpw;
+  long long tok0 = (long long)(blockIdx.x * (QR_THREADS / 32) + me.warp) * me.tpw;
+  QrToken now(p, tok0 + me.tslot);
+  const __nv_bfloat16 *x = now.in_tensor(p.x, me.h0), *dy = now.in_tensor(p.in, me.h0);
+  Packed rx = map.load(x, now.in && me.h0 < p.H), rg = map.load(dy, now.in && me.h0 < p.H);
+  double pos = now.position(p);
+  for (; tok0 < p.tokens; tok0 += step) {
+    const QrToken next(p, tok0 + step + me.tslot);
+    const __nv_bfloat16 *x_next = next.in_tensor(p.x, me.h0), *dy_next = next.in_tensor(p.in, me.h0);
+    __nv_bfloat16* dx = now.in_tensor(p.out, me.h0);
+    turn.set(p, me, pos);
+    pos = next.position(p);
+#pragma unroll 1
+    for (int h = me.h0; h - me.h0 < p.H; h += me.hps) {
+      const Pairs v = unpack<INTER>(rx);
+      Pairs g = unpack<INTER>(rg);
+      x += p.x.sh * me.hps;
+      dy += p.in.sh * me.hps;
+      const bool more = h - me.h0 + me.hps < p.H;       // of the whole warp
+      const bool ok = more ? now.in && h + me.hps < p.H : next.in && me.h0 < p.H;
+      rx = map.load(more ? x : x_next, ok);
+      rg = map.load(more ? dy : dy_next, ok);
+      const float rstd = rsqrtf(row_sum<LPR>(dot16(v, v)) * inv_hd + p.eps);
+      turn.rotate(g, me);
+      // du * xhat, for the weights; rows that are not there add zeros
+      if (h < p.n_q) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
-      const float rstd = rsqrtf(row_sum<LPR>(ss) / (float)p.hd + p.eps);
-      rotate<INTER>(g, cs, sn);
-      float dot = 0.f;
+        for (int j = 0; j < 4; ++j) { dq.a[j] = ffma2(fmul2(g.a[j], both(rstd)), v.a[j], dq.a[j]); dq.b[j] = ffma2(fmul2(g.b[j], both(rstd)), v.b[j], dq.b[j]); }
+      } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        v[i] *= rstd;
-        const float d = g[i] * v[i];                       // rows that are not there add zeros
-        if (is_q) dq[i] += d; else dk[i] += d;
-        g[i] *= is_q ? wq[i] : wk[i];
-        dot = fmaf(g[i], v[i], dot);
+        for (int j = 0; j < 4; ++j) { dk.a[j] = ffma2(fmul2(g.a[j], both(rstd)), v.a[j], dk.a[j]); dk.b[j] = ffma2(fmul2(g.b[j], both(rstd)), v.b[j], dk.b[j]); }
       }
-      dot = row_sum<LPR>(dot) / (float)p.hd;
+      weights.times(g, h < p.n_q ? 0 : 1, me.l);
+      // dx = rstd (g - xhat mean(g xhat)); the factors of x in an order that cannot overflow: (rstd x) has mean square 1
+      const float back = -row_sum<LPR>(dot16(g, v)) * rstd * inv_hd;
+      Pairs out;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = rstd * (g[i] - v[i] * dot);
-      if (ok) store_row<INTER, VEC>(dx + h * p.out.sh, l, p.hd, p.n_freq, v);
+      for (int j = 0; j < 4; ++j) {
+        out.a[j] = ffma2(fmul2(v.a[j], both(rstd)), both(back), g.a[j]);
+        out.b[j] = ffma2(fmul2(v.b[j], both(rstd)), both(back), g.b[j]);
+      }
+      scale_by(out, rstd);
+      if (now.in && h < p.H) map.store(dx, pack<INTER>(out));
+      dx += p.out.sh * me.hps;
     }
+    now = next;
+    x = x_next;
+    dy = dy_next;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 16; ++i) {                        // pair i % 8, first elements then second ones
+    float2 &fq = i < 8 ? dq.a[i / 2] : dq.b[i / 2 - 4], &fk = i < 8 ? dk.a[i / 2] : dk.b[i / 2 - 4];
+    float sq = i & 1 ? fq.y : fq.x, sk = i & 1 ? fk.y : fk.x;
 #pragma unroll
     for (int o = LPR; o < 32; o <<= 1) {
-      dq[i] += __shfl_xor_sync(0xffffffffu, dq[i], o);
-      dk[i] += __shfl_xor_sync(0xffffffffu, dk[i], o);
+      sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      sk += __shfl_xor_sync(0xffffffffu, sk, o);
     }
-    if (slot == 0) { sums[warp][0][l * 16 + i] = dq[i]; sums[warp][1][l * 16 + i] = dk[i]; }
+    if (me.lane < LPR) { sums[me.warp][0][me.l * 16 + i] = sq; sums[me.warp][1][me.l * 16 + i] = sk; }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * LPR * 16; i += QR_THREADS) {
-    const int which = i / (LPR * 16), at = i % (LPR * 16), lane_of = at / 16, k = at % 16;
-    const int pair = 8 * lane_of + (INTER ? k / 2 : k % 8);
+    const int which = i / (LPR * 16), at = i % (LPR * 16), pair = 8 * (at / 16) + at % 8;
     if (2 * pair >= p.hd) continue;
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < QR_THREADS / 32; ++w) s += sums[w][which][at];
-    int a, bb;
-    pair_at<INTER>(pair, p.hd, p.n_freq, a, bb);
-    const bool second = INTER ? (k & 1) : k >= 8;
-    p.part[((long long)blockIdx.x * 2 + which) * p.hd + (second ? bb : a)] = s;
+    int a, b;
+    pair_at<INTER>(pair, p.hd, p.n_freq, a, b);
+    p.part[((long long)blockIdx.x * 2 + which) * p.hd + (at % 16 < 8 ? a : b)] = s;
   }
 }
 
-// dw[which][c] += sum over blocks of part[block][which][c]; 32 columns a block, eight runs of blocks each. One thread adds to both
-// weights, which may be the same.
-__global__ void qk_norm_dw_kernel(const float* part, int blocks, int hd, float* dwq, float* dwk) {
+// dw[which][c] += sum over blocks of part[block][which][c]; 8 columns a block, 32 runs of blocks each (with 32 columns and eight runs
+// 592 blocks took 33 us, one load after the other). One thread adds to both weights, which may be the same.
+__global__ void __launch_bounds__(256)
+qk_norm_dw_kernel(const float* part, int blocks, int hd, float* dwq, float* dwk) {
   griddep_wait();
   griddep_launch();
-  __shared__ float s[8][2][32];
-  const int col = threadIdx.x & 31, c = blockIdx.x * 32 + col, run = threadIdx.x >> 5;
+  __shared__ float s[32][2][8];
+  const int col = threadIdx.x & 7, c = blockIdx.x * 8 + col, run = threadIdx.x >> 3;
   float a = 0.f, b = 0.f;
-  if (c < hd)
-    for (int i = run; i < blocks; i += 8) {
+  if (c < hd) {
+#pragma unroll 4
+    for (int i = run; i < blocks; i += 32) {
       a += part[(long long)i * 2 * hd + c];
       b += part[(long long)i * 2 * hd + hd + c];
     }
+  }
   s[run][0][col] = a;
   s[run][1][col] = b;
   __syncthreads();
   if (run == 0 && c < hd) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) { a += s[i][0][col]; b += s[i][1][col]; }
+    for (int i = 1; i < 32; ++i) { a += s[i][0][col]; b += s[i][1][col]; }
     dwq[c] += a;
     dwk[c] += b;
   }
@@ -270,19 +403,19 @@ static int qr_blocks(const QrParams& p, int lpr, int per_sm) {
   return (int)(need < (long long)num_sms() * per_sm ? need : (long long)num_sms() * per_sm);
 }
 
-constexpr int QR_BWD_PER_SM = 4;
+constexpr int QR_FWD_PER_SM = 4, QR_BWD_PER_SM = 2;
 
 template <int LPR, bool INTER, bool VEC>
 static int qr_launch(const QrParams& p, bool norm, bool bwd, float* dwq, float* dwk, cudaStream_t st) {
   if (!bwd) {
-    const int grid = qr_blocks(p, LPR, 16);
+    const int grid = qr_blocks(p, LPR, QR_FWD_PER_SM);
     return launch_overlapped(norm ? qk_rotary_fwd_kernel<LPR, INTER, VEC, true> : qk_rotary_fwd_kernel<LPR, INTER, VEC, false>,
                              dim3(grid), dim3(QR_THREADS), 0, st, 1, p);
   }
   const int grid = qr_blocks(p, LPR, QR_BWD_PER_SM);
   const int e = launch_overlapped(qk_norm_rotary_bwd_kernel<LPR, INTER, VEC>, dim3(grid), dim3(QR_THREADS), 0, st, 1, p);
   if (e) return e;
-  return launch_overlapped(qk_norm_dw_kernel, dim3((p.hd + 31) / 32), dim3(256), 0, st, 1, (const float*)p.part, grid, p.hd, dwq, dwk);
+  return launch_overlapped(qk_norm_dw_kernel, dim3((p.hd + 7) / 8), dim3(256), 0, st, 1, (const float*)p.part, grid, p.hd, dwq, dwk);
 }
 
 template <bool INTER, bool VEC>
