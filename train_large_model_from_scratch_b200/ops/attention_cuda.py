@@ -124,8 +124,46 @@ def bwd(do, qkv, o, lse, n_q: int, n_kv: int, causal: bool, rope=None):
 def _tiled(t: torch.Tensor) -> torch.Tensor:
     """`t [B, T, H, hd]` as tiles can be loaded from it: rows contiguous, 16-byte aligned, at strides of whole 16 bytes. Anything
     else is copied (a broadcast tensor, an odd slice)."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in t.stride()[:3])
+    b, r, h, c = t.stride()
+    ok = c == 1 and t.data_ptr() % 16 == 0 and b > 0 and r > 0 and h > 0 and (b | r | h) % 8 == 0
     return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _window_fwd(q: int, k: int, v: int, strides, B: int, T: int, n_q: int, n_kv: int, hd: int, window: int, sinks: int, device):
+    o = torch.empty((B, T, n_q, hd), dtype=torch.bfloat16, device=device)
+    lse = torch.empty((B, n_q, T), dtype=torch.float32, device=device)
+    native._check(native.lib().tlm_attn_window_fwd(q, k, v, strides, o.data_ptr(), lse.data_ptr(), B, T, n_q, n_kv, hd,
+                                                   1.0 / math.sqrt(hd), min(window, T), min(sinks, T), native._stream()), "attn_window_fwd")
+    return o, lse
+
+
+def _window_bwd(do, q: int, k: int, v: int, strides, o, lse, dq: int, dk: int, dv: int, out_strides, B: int, T: int, n_q: int, n_kv: int,
+                hd: int, window: int, sinks: int, rope) -> None:
+    do = _aligned(do)
+    window, sinks = min(window, T), min(sinks, T)
+    l = native.lib()
+    rows = B * n_q * T                                       # scratch: dQ in fp32, sums of the sink rows, delta
+    part = rows * hd
+    delta = part + l.tlm_attn_window_part_floats(B, T, n_kv, hd, window, sinks)
+    work = torch.empty(delta + rows, dtype=torch.float32, device=do.device)
+    w = work.data_ptr()
+    cos, sin = (t.data_ptr() for t in rope) if rope is not None else (None, None)
+    native._check(l.tlm_attn_window_bwd(q, k, v, strides, o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq, dk, dv, out_strides, w,
+                                        w + 4 * delta, w + 4 * part, B, T, n_q, n_kv, hd, 1.0 / math.sqrt(hd), cos, sin, window, sinks,
+                                        native._stream()), "attn_window_bwd")
+
+
+def _packed(qkv: torch.Tensor, n_q: int, n_kv: int):
+    """Addresses of the q, k and v heads of a packed tensor, and their strides (the same three times)."""
+    s = qkv.stride()[:3]
+    head = qkv.element_size() * s[2]
+    p = qkv.data_ptr()
+    return p, p + n_q * head, p + (n_q + n_kv) * head, native._LL9(*s, *s, *s)
 
 
 def window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int):
@@ -133,29 +171,30 @@ def window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, s
     `window` keys, itself included (0: all), and the first `sinks`. -> o `[B, T, Hq, hd]` bf16, lse `[B, Hq, T]` fp32."""
     q, k, v = _tiled(q), _tiled(k), _tiled(v)
     B, T, n_q, hd = q.shape
-    o = torch.empty(B, T, n_q, hd, dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty(B, n_q, T, dtype=torch.float32, device=q.device)
-    native._check(native.lib().tlm_attn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), native._strides(q, k, v), o.data_ptr(),
-                                                   lse.data_ptr(), B, T, n_q, k.shape[2], hd, 1.0 / math.sqrt(hd), min(window, T),
-                                                   min(sinks, T), native._stream()), "attn_window_fwd")
-    return o, lse
+    strides = native._LL9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    return _window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, B, T, n_q, k.shape[2], hd, window, sinks, q.device)
+
+
+def window_fwd_packed(qkv: torch.Tensor, n_q: int, n_kv: int, window: int, sinks: int):
+    """The same on the heads of `qkv [B, T, n_q + 2 n_kv, hd]`."""
+    qkv = _tiled(qkv)
+    B, T, _, hd = qkv.shape
+    return _window_fwd(*_packed(qkv, n_q, n_kv), B, T, n_q, n_kv, hd, window, sinks, qkv.device)
 
 
 def window_bwd(do, q, k, v, o, lse, window: int, sinks: int, out, rope=None) -> None:
     """Gradients of `window_fwd` into `out = (dq, dk, dv)` (bf16, rows contiguous, 16-byte aligned). `rope`: as in `bwd`."""
     q, k, v = _tiled(q), _tiled(k), _tiled(v)
-    do = do.contiguous()
-    if do.data_ptr() % 16:
-        do = do.clone()
     B, T, n_q, hd = q.shape
-    n_kv = k.shape[2]
-    f32 = dict(dtype=torch.float32, device=q.device)
-    dq_acc, delta = torch.empty(B, n_q, T, hd, **f32), torch.empty(B, n_q, T, **f32)
-    window, sinks = min(window, T), min(sinks, T)
-    n_part = native.lib().tlm_attn_window_part_floats(B, T, n_kv, hd, window, sinks)
-    part = torch.empty(n_part, **f32) if n_part else None
-    cos, sin = rope if rope is not None else (None, None)
-    native._check(native.lib().tlm_attn_window_bwd(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), native._strides(q, k, v), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-        *(t.data_ptr() for t in out), native._strides(*out), dq_acc.data_ptr(), delta.data_ptr(), native._ptr(part), B, T, n_q, n_kv,
-        hd, 1.0 / math.sqrt(hd), native._ptr(cos), native._ptr(sin), window, sinks, native._stream()), "attn_window_bwd")
+    strides, out_strides = (native._LL9(*a.stride()[:3], *b.stride()[:3], *c.stride()[:3]) for a, b, c in ((q, k, v), out))
+    _window_bwd(do, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o, lse, *(t.data_ptr() for t in out), out_strides, B, T, n_q,
+                k.shape[2], hd, window, sinks, rope)
+
+
+def window_bwd_packed(do, qkv, o, lse, n_q: int, n_kv: int, window: int, sinks: int, rope=None) -> torch.Tensor:
+    """-> gradient of the packed tensor."""
+    qkv = _tiled(qkv)
+    B, T, H, hd = qkv.shape
+    dqkv = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=qkv.device)
+    _window_bwd(do, *_packed(qkv, n_q, n_kv), o, lse, *_packed(dqkv, n_q, n_kv), B, T, n_q, n_kv, hd, window, sinks, rope)
+    return dqkv

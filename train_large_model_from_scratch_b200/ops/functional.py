@@ -323,7 +323,9 @@ def attention_packed(qkv: torch.Tensor, n_q: int, n_kv: int, causal: bool = True
         raise ValueError("a window needs causal attention")
     if qkv.dim() != 4 or qkv.shape[2] != n_q + 2 * n_kv:
         raise ValueError(f"qkv has to be [B, T, {n_q + 2 * n_kv}, hd], not {tuple(qkv.shape)}")
-    _check_window(*_heads_of(qkv, n_q, n_kv), window, sinks)
+    _check_window(qkv, n_q, n_kv, window, sinks)
+    if not (qkv.requires_grad and torch.is_grad_enabled()):
+        return _window_packed_fwd(qkv, n_q, n_kv, window, sinks)[0]
     return _WindowPacked.apply(qkv, n_q, n_kv, window, sinks)
 
 
@@ -332,28 +334,25 @@ def _heads_of(qkv, n_q, n_kv):
     return qkv[:, :, :n_q], qkv[:, :, n_q:n_q + n_kv], qkv[:, :, n_q + n_kv:]
 
 
-def _check_device(*tensors) -> None:
+def _check_device(x, *others) -> None:
     """CUDA tensors of one call lie on the current device, whose stream the kernels are issued to."""
-    dev = tensors[0].device
-    if any(t.device != dev for t in tensors):
-        raise ValueError("tensors on different devices: " + ", ".join(str(t.device) for t in tensors))
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}: "
-                         f"call under torch.cuda.device({dev.index})")
+    dev = x.get_device()                                     # -1: the CPU
+    for t in others:
+        if t.get_device() != dev:
+            raise ValueError("tensors on different devices: " + ", ".join(str(t.device) for t in (x, *others)))
+    if dev >= 0 and dev != torch.cuda.current_device():
+        raise ValueError(f"tensors on cuda:{dev}, but the current device is cuda:{torch.cuda.current_device()}: "
+                         f"call under torch.cuda.device({dev})")
 
 
-def _check_window(q, k, v, window, sinks) -> None:
-    if q.dim() != 4 or k.shape != v.shape or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"q [B, T, Hq, hd] with k and v [B, T, Hkv, hd] expected, not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f"the number of query heads ({q.shape[2]}) has to be a multiple of the number of KV heads ({k.shape[2]})")
+def _check_window(x, n_q, n_kv, window, sinks, *others) -> None:
+    if n_kv <= 0 or n_q <= 0 or n_q % n_kv:
+        raise ValueError(f"the number of query heads ({n_q}) has to be a multiple of the number of KV heads ({n_kv})")
     if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
         raise ValueError(f"window {window}, sinks {sinks}: neither may be negative, and sinks need a window")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
-        raise ValueError(f"q, k and v of one type expected, not {q.dtype}, {k.dtype}, {v.dtype}")
-    _check_device(q, k, v)
-    if _use_native(q) and q.shape[3] not in (32, 64, 128):
-        raise ValueError(f"head dim {q.shape[3]}: the window kernels have 32, 64 and 128")
+    _check_device(x, *others)
+    if _use_native(x) and x.shape[3] not in (32, 64, 128):
+        raise ValueError(f"head dim {x.shape[3]}: the window kernels have 32, 64 and 128")
 
 
 class _Window(torch.autograd.Function):
@@ -379,16 +378,18 @@ class _Window(torch.autograd.Function):
         return *out, None, None
 
 
+def _window_packed_fwd(qkv, n_q, n_kv, window, sinks):
+    if _use_native(qkv):
+        return native.window_attn_fwd_packed(qkv, n_q, n_kv, window, sinks)
+    o, lse, *_ = _attn_fwd_ref(*_heads_of(qkv, n_q, n_kv), True, window, sinks)
+    return o.to(qkv.dtype).contiguous(), lse
+
+
 class _WindowPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, n_q, n_kv, window, sinks):
         ctx.meta = (n_q, n_kv, window, sinks)
-        q, k, v = _heads_of(qkv, n_q, n_kv)
-        if _use_native(qkv):
-            o, lse = native.window_attn_fwd(q, k, v, window, sinks)
-        else:
-            o, lse, *_ = _attn_fwd_ref(q, k, v, True, window, sinks)
-            o = o.to(qkv.dtype).contiguous()
+        o, lse = _window_packed_fwd(qkv, n_q, n_kv, window, sinks)
         ctx.save_for_backward(qkv, o, lse)
         return o
 
@@ -396,12 +397,10 @@ class _WindowPacked(torch.autograd.Function):
     def backward(ctx, do):
         qkv, o, lse = ctx.saved_tensors
         n_q, n_kv, window, sinks = ctx.meta
-        q, k, v = _heads_of(qkv, n_q, n_kv)
         if _use_native(qkv):
-            dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-            native.window_attn_bwd(do, q, k, v, o, lse, window, sinks, _heads_of(dqkv, n_q, n_kv))
+            dqkv = native.window_attn_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks)
         else:
-            dqkv = torch.cat(_attn_bwd_ref(do, q, k, v, o, True, window, sinks), dim=2).to(qkv.dtype)
+            dqkv = torch.cat(_attn_bwd_ref(do, *_heads_of(qkv, n_q, n_kv), o, True, window, sinks), dim=2).to(qkv.dtype)
         return dqkv, None, None, None, None
 
 
@@ -411,7 +410,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     packed tensor; rows that are no whole 16-byte pieces apart are copied first. bf16 on the GPU with head dims 32, 64, 128.
     Inputs have to be finite where a row's 128 neighbours look: a hidden key's weight is exactly zero, but zero times an infinite
     or NaN value is NaN."""
-    _check_window(q, k, v, window, sinks)
+    if q.dim() != 4 or k.shape != v.shape or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"q [B, T, Hq, hd] with k and v [B, T, Hkv, hd] expected, not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"q, k and v of one type expected, not {q.dtype}, {k.dtype}, {v.dtype}")
+    _check_window(q, q.shape[2], k.shape[2], window, sinks, k, v)
     return _Window.apply(q, k, v, window, sinks)
 
 
@@ -434,60 +437,84 @@ def _check_rotary(x, positions, inv_freq) -> tuple[torch.Tensor, torch.Tensor, t
     return x, positions.contiguous(), inv_freq.contiguous()
 
 
+class _Turn:
+    """What a rotation needs besides its tensor, unchanged between forward and backward."""
+    __slots__ = ("positions", "inv_freq", "interleaved", "scale", "versions")
+
+    def __init__(self, positions, inv_freq, interleaved, scale):
+        self.positions, self.inv_freq, self.interleaved, self.scale = positions, inv_freq, bool(interleaved), float(scale)
+        self.versions = None
+
+    def keep(self):
+        if not (self.positions.is_inference() or self.inv_freq.is_inference()):
+            self.versions = (self.positions._version, self.inv_freq._version)
+
+    def check(self):
+        if self.versions is not None and self.versions != (self.positions._version, self.inv_freq._version):
+            raise RuntimeError("positions or inv_freq have been modified in place since the forward pass")
+
+
+def _turn(x, turn: _Turn, inverse: bool = False):
+    if _use_native(x):
+        return native.qk_rotary(x, turn.positions, turn.inv_freq, interleaved=turn.interleaved, scale=turn.scale, inverse=inverse)
+    return oracle.rotary(x, turn.positions, turn.inv_freq, turn.interleaved, turn.scale, inverse).to(x.dtype)
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, positions, inv_freq, interleaved, scale):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.meta = (interleaved, scale)
-        return _Rotary.turn(x, positions, inv_freq, interleaved, scale, False)
-
-    @staticmethod
-    def turn(x, positions, inv_freq, interleaved, scale, inverse):
-        if _use_native(x):
-            return native.qk_rotary(x, positions, inv_freq, interleaved=interleaved, scale=scale, inverse=inverse)
-        return oracle.rotary(x, positions, inv_freq, interleaved, scale, inverse).to(x.dtype)
+    def forward(ctx, x, turn):
+        ctx.turn = turn
+        turn.keep()
+        return _turn(x, turn)
 
     @staticmethod
     def backward(ctx, dy):
-        return _Rotary.turn(dy.contiguous(), *ctx.saved_tensors, *ctx.meta, True), None, None, None, None
+        ctx.turn.check()
+        return _turn(dy.contiguous(), ctx.turn, inverse=True), None
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
     """Every head of `x [B, T, H, hd]` turned by its token's position: `positions` int64 `[T]` or `[B, T]` (any values), `inv_freq`
     and `scale` from `oracle.rotary_frequencies`. The first `2 * len(inv_freq)` elements of a head turn, in pairs
     (i, i + len(inv_freq)) or, `interleaved`, (2 i, 2 i + 1); the rest passes. A new tensor; `x` may be a view (rows contiguous)."""
-    return _Rotary.apply(*_check_rotary(x, positions, inv_freq), bool(interleaved), float(scale))
+    x, positions, inv_freq = _check_rotary(x, positions, inv_freq)
+    turn = _Turn(positions, inv_freq, interleaved, scale)
+    return _Rotary.apply(x, turn) if x.requires_grad and torch.is_grad_enabled() else _turn(x, turn)
 
 
 class _QkNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, n_q, q_weight, k_weight, positions, inv_freq, eps, interleaved, scale):
-        ctx.save_for_backward(x, positions, inv_freq)
-        ctx.weights, ctx.meta = (q_weight, k_weight), (n_q, eps, interleaved, scale)
-        return _qk_norm_fwd(x, ctx.weights, positions, inv_freq, *ctx.meta)
+    def forward(ctx, x, q_weight, k_weight, n_q, eps, turn):
+        ctx.save_for_backward(x)
+        ctx.weights, ctx.n_q, ctx.eps, ctx.turn = (q_weight, k_weight), n_q, eps, turn
+        turn.keep()
+        return _qk_norm_fwd(x, ctx.weights, n_q, eps, turn)
 
     @staticmethod
     def backward(ctx, dy):
-        return _qk_norm_bwd(dy.contiguous(), *ctx.saved_tensors, ctx.weights, *ctx.meta), *[None] * 8
+        (x,) = ctx.saved_tensors
+        ctx.turn.check()
+        return _qk_norm_bwd(dy.contiguous(), x, ctx.weights, ctx.n_q, ctx.eps, ctx.turn), None, None, None, None, None
 
 
-def _qk_norm_fwd(x, weights, positions, inv_freq, n_q, eps, interleaved, scale):
+def _qk_norm_fwd(x, weights, n_q, eps, turn):
     if _use_native(x):
-        return native.qk_rotary(x, positions, inv_freq, weights, n_q, eps, interleaved, scale)
+        return native.qk_rotary(x, turn.positions, turn.inv_freq, weights, n_q, eps, turn.interleaved, turn.scale)
     xf = x.float()
     hat = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
     u = torch.cat([hat[:, :, :n_q] * weights[0].float(), hat[:, :, n_q:] * weights[1].float()], dim=2)
-    return oracle.rotary(u, positions, inv_freq, interleaved, scale).to(x.dtype)
+    return oracle.rotary(u, turn.positions, turn.inv_freq, turn.interleaved, turn.scale).to(x.dtype)
 
 
-def _qk_norm_bwd(dy, x, positions, inv_freq, weights, n_q, eps, interleaved, scale, out=None):
-    grads = [_main_grad(w) for w in weights]
+def _qk_norm_bwd(dy, x, weights, n_q, eps, turn, out=None):
+    """Gradient of `x` (into `out`, which may be `dy`); those of the weights are added to their `main_grad`."""
+    grads = (_main_grad(weights[0]), _main_grad(weights[1]))
     if _use_native(x):
-        return native.qk_norm_rotary_bwd(dy, x, positions, inv_freq, weights, grads, n_q, eps, interleaved, scale, out)
+        return native.qk_norm_rotary_bwd(dy, x, turn.positions, turn.inv_freq, weights, grads, n_q, eps, turn.interleaved, turn.scale, out)
     xf = x.float()
     rstd = torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
     hat = xf * rstd
-    du = oracle.rotary(dy, positions, inv_freq, interleaved, scale, inverse=True)
+    du = oracle.rotary(dy, turn.positions, turn.inv_freq, turn.interleaved, turn.scale, inverse=True)
     g = torch.empty_like(du)
     for w, mg, heads in zip(weights, grads, (slice(0, n_q), slice(n_q, None))):
         mg.add_((du[:, :, heads] * hat[:, :, heads]).sum((0, 1, 2)))
@@ -507,7 +534,10 @@ def qk_norm_rotary(x: torch.Tensor, n_q: int, q_weight: torch.Tensor, k_weight: 
         if tuple(w.shape) != (x.shape[3],) or w.dtype != x.dtype or not w.is_contiguous():
             raise ValueError(f"weights have to be contiguous {x.dtype} [{x.shape[3]}], not {w.dtype} {tuple(w.shape)}")
     _check_device(x, q_weight, k_weight)
-    return _QkNormRotary.apply(x, n_q, q_weight, k_weight, positions, inv_freq, float(eps), bool(interleaved), float(scale))
+    n_q, eps, turn = int(n_q), float(eps), _Turn(positions, inv_freq, interleaved, scale)
+    if torch.is_grad_enabled() and (x.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+        return _QkNormRotary.apply(x, q_weight, k_weight, n_q, eps, turn)
+    return _qk_norm_fwd(x, (q_weight, k_weight), n_q, eps, turn)
 
 
 # --------------------------------------------------------------------------- SwiGLU

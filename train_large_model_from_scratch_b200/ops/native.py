@@ -130,7 +130,8 @@ def _declare(l) -> None:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the handle alone: a `torch.cuda.Stream` object around it costs 3 us a call
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _check(code: int, what: str) -> None:
@@ -430,10 +431,7 @@ def rope_qk(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot: int,
     return qkv
 
 
-def _strides(*tensors: torch.Tensor):
-    """Batch, token and head strides of `[B, T, H, hd]` tensors, in elements."""
-    flat = [s for t in tensors for s in t.stride()[:3]]
-    return (ctypes.c_longlong * len(flat))(*flat)
+_LL3, _LL9 = _c.c_longlong * 3, _c.c_longlong * 9
 
 
 def qk_rotary(x, positions, inv_freq, weights=None, n_q: int = 0, eps: float = 0.0, interleaved: bool = False, scale: float = 1.0,
@@ -441,11 +439,11 @@ def qk_rotary(x, positions, inv_freq, weights=None, n_q: int = 0, eps: float = 0
     """`x [B, T, H, hd]` bf16 (rows contiguous) rotated by `positions` (int64, `[T]` or `[B, T]`) and `inv_freq` (float64), with
     `weights = (q, k)` behind an RMS norm of every head (`csrc/qk_rotary.cu`). `inverse`: the transposed rotation, without norm."""
     B, T, H, hd = x.shape
-    y = torch.empty(B, T, H, hd, dtype=torch.bfloat16, device=x.device)
-    wq, wk = weights if weights is not None else (None, None)
-    _check(lib().tlm_qk_rotary(x.data_ptr(), _strides(x), y.data_ptr(), _strides(y), positions.data_ptr(),
-                               T if positions.dim() > 1 else 0, inv_freq.data_ptr(), inv_freq.numel(), _ptr(wq), _ptr(wk), B, T, H,
-                               n_q, hd, eps, scale, int(interleaved), int(inverse), _stream()), "qk_rotary")
+    y = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=x.device)
+    wq, wk = (w.data_ptr() for w in weights) if weights is not None else (None, None)
+    _check(lib().tlm_qk_rotary(x.data_ptr(), _LL3(*x.stride()[:3]), y.data_ptr(), _LL3(T * H * hd, H * hd, hd), positions.data_ptr(),
+                               T if positions.dim() > 1 else 0, inv_freq.data_ptr(), inv_freq.shape[0], wq, wk, B, T, H, n_q, hd, eps,
+                               scale, interleaved, inverse, _stream()), "qk_rotary")
     return y
 
 
@@ -454,13 +452,13 @@ def qk_norm_rotary_bwd(dy, x, positions, inv_freq, weights, grads, n_q: int, eps
     `dy` itself."""
     B, T, H, hd = x.shape
     if out is None:
-        out = torch.empty(B, T, H, hd, dtype=torch.bfloat16, device=x.device)
+        out = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=x.device)
     work = torch.empty(lib().tlm_qk_norm_work_floats(hd), dtype=torch.float32, device=x.device)
-    _check(lib().tlm_qk_norm_rotary_bwd(x.data_ptr(), _strides(x), dy.data_ptr(), _strides(dy), out.data_ptr(), _strides(out),
-                                        positions.data_ptr(), T if positions.dim() > 1 else 0, inv_freq.data_ptr(), inv_freq.numel(),
-                                        weights[0].data_ptr(), weights[1].data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(),
-                                        work.data_ptr(), B, T, H, n_q, hd, eps, scale, int(interleaved), _stream()),
-           "qk_norm_rotary_bwd")
+    _check(lib().tlm_qk_norm_rotary_bwd(x.data_ptr(), _LL3(*x.stride()[:3]), dy.data_ptr(), _LL3(*dy.stride()[:3]), out.data_ptr(),
+                                        _LL3(*out.stride()[:3]), positions.data_ptr(), T if positions.dim() > 1 else 0,
+                                        inv_freq.data_ptr(), inv_freq.shape[0], weights[0].data_ptr(), weights[1].data_ptr(),
+                                        grads[0].data_ptr(), grads[1].data_ptr(), work.data_ptr(), B, T, H, n_q, hd, eps, scale,
+                                        interleaved, _stream()), "qk_norm_rotary_bwd")
     return out
 
 
@@ -573,9 +571,19 @@ def window_attn_fwd(q, k, v, window: int, sinks: int):
     return attention_cuda.window_fwd(q, k, v, window, sinks)
 
 
+def window_attn_fwd_packed(qkv, n_q: int, n_kv: int, window: int, sinks: int):
+    from . import attention_cuda
+    return attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks)
+
+
 def window_attn_bwd(do, q, k, v, o, lse, window: int, sinks: int, out, rope=None) -> None:
     from . import attention_cuda
     attention_cuda.window_bwd(do, q, k, v, o, lse, window, sinks, out, rope)
+
+
+def window_attn_bwd_packed(do, qkv, o, lse, n_q: int, n_kv: int, window: int, sinks: int, rope=None) -> torch.Tensor:
+    from . import attention_cuda
+    return attention_cuda.window_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks, rope)
 
 
 # --------------------------------------------------------------------------- grouped GEMMs (MoE experts)
