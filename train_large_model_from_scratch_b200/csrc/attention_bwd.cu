@@ -28,13 +28,10 @@
 // dV | dK rows meet the tile's own in an fp32 buffer that the conversion pass adds up in fixed order.
 // Every wait is bounded; on a timeout the CTA records a status code, leaves its
 // loops and still releases its tensor memory.
-#include "common.cuh"
-#include "window_plan.h"
+#include "attention_window.h"
 #include <cstdlib>
 
 namespace tlm {
-
-int make_bthd_map(CUtensorMap* map, const void* base, const long long* strides, int B, int T, int heads, int hd, int box_rows, int box_cols);
 
 constexpr int AB_TILE = 128, AB_THREADS = 704, AB_MAX_DST = 8;
 
@@ -394,16 +391,17 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
   const int split = SPLIT ? p.split : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
   int q_from, q_to, part = -1;                                // query tiles; slot of `part` that this block's sink rows go to
   if constexpr (WIN) {
-    // the far pieces first: they are as long as the others, and the last blocks should not be theirs
-    const int item = (int)blockIdx.x / split, far_items = p.far.tiles * p.far.chunks * p.B * p.Hkv;
-    if (item < far_items) {
-      const int c = item % p.far.chunks, r = item / p.far.chunks;
-      j = r % p.far.tiles;
-      bh = r / p.far.tiles;
+    // A head's far pieces come in front of its tiles: they are as long, and what they read is read again by the group's tiles
+    const int far_items = p.far.tiles * p.far.chunks;
+    int rank;
+    heavy_first_decode((int)blockIdx.x / split, n_tiles + far_items, p.B * p.Hkv, p.head_group, rank, bh);
+    if (rank < far_items) {
+      const int c = rank / p.far.tiles;
+      j = rank - c * p.far.tiles;
       win_far_range(p.far, j, c, p.window, n_tiles, q_from, q_to);
       part = 1 + c;
     } else {
-      heavy_first_decode(item - far_items, n_tiles, p.B * p.Hkv, p.head_group, j, bh);
+      j = rank - far_items;
       q_from = j;
       q_to = win_last_q(j, p.window, n_tiles) + 1;
       if (j < p.far.tiles) part = 0;
@@ -419,6 +417,9 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
   const int it0 = SPLIT ? rep * per_head * rank / split : 0;                                       // this CTA's steps
   const int n_it = SPLIT ? rep * per_head * (rank + 1) / split - it0 : rep * per_head;             // (SPLIT: may be none)
   const int heads_total = p.Hq + 2 * p.Hkv;
+  // query head and query tile of this CTA's first step; a step further is the next tile, behind the last one the next head's first
+  const int hq0 = kvh * rep + (n_it > 0 ? it0 / per_head : 0), qi0 = q_from + (n_it > 0 ? it0 % per_head : 0);
+  auto advance = [&](int& hq, int& qi) { if (++qi == q_to) { qi = q_from; ++hq; } };
   const CUtensorMap *tm_q, *tm_k, *tm_v;
   int k_head = kvh, v_head = kvh;
   if constexpr (WIN) { tm_q = &tm.q; tm_k = &tm.k; tm_v = &tm.v; }
@@ -453,9 +454,8 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
         if (!C::KV_TMEM) tma_load_4d(sbase + C::OFF_V + kb * 16384, tm_v, bar(KV_FULL), kb * 64, v_head, j * AB_TILE, b);
       }
     }
-    for (int it = 0; it < n_it; ++it) {
+    for (int it = 0, hq = hq0, qi = qi0; it < n_it; ++it, advance(hq, qi)) {
       const int st = it % C::STAGES;
-      const int hq = kvh * rep + (it0 + it) / per_head, qi = q_from + (it0 + it) % per_head;
       if (!mbar_wait_warp(bar(RING_EMPTY + st), ((uint32_t)(it / C::STAGES) & 1u) ^ 1u, 21, abort_flag, p.status)) break;
       if (lane == 0) {
         mbar_expect_tx(bar(RING_FULL + st), (C::WIDE ? 1 : 2) * C::TILE_BYTES);
@@ -652,8 +652,8 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
     }
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     const int col0 = (g & 1) * 32;                             // of the half's 64 query columns
-    for (int it = 0; it < n_it; ++it) {
-      const int st = it % C::STAGES, qi = q_from + (it0 + it) % per_head;
+    for (int it = 0, hq = hq0, qi = qi0; it < n_it; ++it, advance(hq, qi)) {
+      const int st = it % C::STAGES;
       const float* rows = reinterpret_cast<const float*>(sal + C::OFF_ROW) + st * 2 * AB_TILE + s * 64 + col0;
       uint8_t* drow = sal + C::OFF_DS + (C::WIDE ? 0 : it & 1) * C::DS_BYTES + s * 16384 + row * 128;
       if (!mbar_wait_warp(bar(RING_FULL + st), (uint32_t)(it / C::STAGES) & 1u, 28, abort_flag, p.status)) { ok = false; break; }
@@ -714,19 +714,13 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
       else tmem_ld32(t_lane + col, r);
       tmem_ld_wait();
     };
-    if (ok && !SPLIT) {
+    if (ok && !SPLIT && !WIN) {
       // dV, dK accumulators -> bf16 rows of the packed gradient tensor
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const float osc = which == 0 ? 1.f : p.scale;
         __nv_bfloat16* dst = p.dqkv + (((long long)b * p.T + t_row) * heads_total + (which == 0 ? p.Hq + p.Hkv : p.Hq) + kvh) * p.hd + out0;
         bool dst_ok = t_row < p.T && out0 < p.hd;
-        float* part_dst = nullptr;
-        if constexpr (WIN) {
-          dst = which == 0 ? p.dv + b * p.dvs[0] + t_row * p.dvs[1] + kvh * p.dvs[2] + out0 : p.dk + b * p.dks[0] + t_row * p.dks[1] + kvh * p.dks[2] + out0;
-          if (part >= 0 && t_row < p.sinks) part_dst = part_row(t_row) + which * HD + out0;
-          else if (part > 0) dst_ok = false;                    // a far piece has nothing for rows behind the sinks
-        }
         if (SCATTER && p.n_dst > 0) {
           const int owner = t_row / p.dst_rows, tl = t_row - owner * p.dst_rows;
           dst_ok = dst_ok && owner < p.n_dst;
@@ -751,11 +745,7 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
             }
           }
         }
-        if (WIN && part_dst != nullptr) {
-#pragma unroll
-          for (int i = 0; i < W; i += 4)
-            *reinterpret_cast<uint4*>(part_dst + i) = n_it > 0 ? make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]) : make_uint4(0, 0, 0, 0);
-        } else if (dst_ok) {
+        if (dst_ok) {
 #pragma unroll
           for (int i = 0; i < W; i += 8) {
             uint4 v;
@@ -765,6 +755,51 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
             v.w = pack_bf16(__uint_as_float(r[i + 6]) * osc, __uint_as_float(r[i + 7]) * osc);
             *reinterpret_cast<uint4*>(dst + i) = v;
           }
+        }
+      }
+    }
+    if constexpr (WIN && !SPLIT) {
+      // dV and dK as bf16 through shared memory (where dS was; every MMA that reads it is done), so that a row leaves in one piece: written
+      // from the accumulators' layout, 16 bytes of 32 rows at a time, it took 3100 cycles. Rows whose sums go to `part` leave as fp32.
+      constexpr int PASSES = C::WIDE ? 2 : 1, CHUNKS = 2 * HD / PASSES / 8;      // 16-byte chunks of a row of the stage
+      uint8_t* stage = sal + C::OFF_DS;
+      const bool summed = part >= 0 && t_row < p.sinks;
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass) {
+#pragma unroll
+        for (int w = 0; w < 2 / PASSES; ++w) {
+          const int which = PASSES == 2 ? pass : w;
+          const float osc = which == 0 ? 1.f : p.scale;
+          uint32_t r[W];
+          load_out((which == 0 ? C::DV_COL : C::DK_COL) + out0, r);
+          if (summed) {
+            uint4* d = reinterpret_cast<uint4*>(part_row(t_row) + which * HD + out0);
+#pragma unroll
+            for (int i = 0; i < W; i += 4) d[i / 4] = n_it > 0 ? make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < W; i += 8) {
+            uint4 v;
+            v.x = pack_bf16(__uint_as_float(r[i]) * osc, __uint_as_float(r[i + 1]) * osc);
+            v.y = pack_bf16(__uint_as_float(r[i + 2]) * osc, __uint_as_float(r[i + 3]) * osc);
+            v.z = pack_bf16(__uint_as_float(r[i + 4]) * osc, __uint_as_float(r[i + 5]) * osc);
+            v.w = pack_bf16(__uint_as_float(r[i + 6]) * osc, __uint_as_float(r[i + 7]) * osc);
+            *reinterpret_cast<uint4*>(stage + row * (CHUNKS * 16) + (((w * HD + out0 + i) / 8 ^ (row & 7)) << 4)) = v;
+          }
+        }
+        __syncwarp();
+        asm volatile("bar.sync 2, 512;" ::: "memory");            // the softmax warps; all of them come here, on an error too
+        if (ok && part <= 0) {
+          for (int i = threadIdx.x - 64; i < AB_TILE * CHUNKS; i += 512) {
+            const int r = i / CHUNKS, ch = i % CHUNKS, t = j * AB_TILE + r, which = PASSES == 2 ? pass : ch * 8 / HD;
+            if (t >= p.T || (part == 0 && t < p.sinks)) continue;
+            __nv_bfloat16* dst = which == 0 ? p.dv + b * p.dvs[0] + t * p.dvs[1] + kvh * p.dvs[2] : p.dk + b * p.dks[0] + t * p.dks[1] + kvh * p.dks[2];
+            *reinterpret_cast<uint4*>(dst + ch * 8 % HD) = *reinterpret_cast<const uint4*>(stage + r * (CHUNKS * 16) + ((ch ^ (r & 7)) << 4));
+          }
+        }
+        if (pass + 1 < PASSES) {
+          __syncwarp();
+          asm volatile("bar.sync 2, 512;" ::: "memory");
         }
       }
     }
@@ -790,8 +825,7 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
     const int q4 = warp & 3;
     const uint32_t t_lane = tmem + ((uint32_t)(q4 * 32) << 16);
     const int box0 = C::OFF_DQS + q4 * C::BOXES * 4096;
-    for (int it = 0; it < n_it; ++it) {
-      const int hq = kvh * rep + (it0 + it) / per_head, qi = q_from + (it0 + it) % per_head;
+    for (int it = 0, hq = hq0, qi = qi0; it < n_it; ++it, advance(hq, qi)) {
       const int y0 = qi * AB_TILE + q4 * 32;                  // first of this warp's 32 query rows
       if (!mbar_wait_warp(bar(DQ_FULL + (C::WIDE ? 0 : it & 1)), (uint32_t)(C::WIDE ? it : it >> 1) & 1u, 32, abort_flag, p.status)) break;
       tc_fence_after();
@@ -1050,12 +1084,11 @@ TLM_API int tlm_attn_window_bwd(const void* q, const void* k, const void* v, con
   const double n_tiles = (T + AB_TILE - 1) / AB_TILE, bh = (double)B * Hkv, rep = Hq / Hkv;
   if ((n_tiles + (double)p.far.tiles * p.far.chunks) * bh * 8 > 2147483647.) return -6;
   AttnBwdMaps<true> maps;
-  const int cols = hd == 32 ? 32 : 64;
   const long long o_strides[3] = {(long long)T * Hq * hd, (long long)Hq * hd, hd};
-  int e = make_bthd_map(&maps.q, q, strides, B, T, Hq, hd, AB_TILE, cols);
-  if (!e) e = make_bthd_map(&maps.k, k, strides + 3, B, T, Hkv, hd, AB_TILE, cols);
-  if (!e) e = make_bthd_map(&maps.v, v, strides + 6, B, T, Hkv, hd, AB_TILE, cols);
-  if (!e) e = make_bthd_map(&maps.dout, dout, o_strides, B, T, Hq, hd, AB_TILE, cols);
+  int e = make_bthd_map(&maps.q, q, strides, B, T, Hq, hd, AB_TILE);
+  if (!e) e = make_bthd_map(&maps.k, k, strides + 3, B, T, Hkv, hd, AB_TILE);
+  if (!e) e = make_bthd_map(&maps.v, v, strides + 6, B, T, Hkv, hd, AB_TILE);
+  if (!e) e = make_bthd_map(&maps.dout, dout, o_strides, B, T, Hq, hd, AB_TILE);
   if (!e) e = make_dq_map(&maps.dq, dq_acc, B, T, Hq, hd);
   if (e) return e;
   e = launch_delta(o, dout, delta, dq_acc, B, T, Hq, hd, st);

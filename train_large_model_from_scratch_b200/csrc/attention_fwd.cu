@@ -20,8 +20,7 @@
 // SM and one CTA's softmax overlaps the other's MMAs. All waits are bounded.
 //
 // WIN, a second instantiation: a sliding window with sinks (see window_plan.h), q, k and v as tensors of their own.
-#include "common.cuh"
-#include "window_plan.h"
+#include "attention_window.h"
 
 namespace tlm {
 
@@ -111,6 +110,12 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
   const int q0 = qt * AT_BQ;
   const int first = WIN ? win_first_tile(qt, p.window) : 0;
   const int n_kv = WIN ? qt - first + 1 + win_sink_tiles(first, p.sinks) : qt + 1;      // causal: KV tiles 0..qt
+  // keys of step j that anybody sees, in whole 16s: of a sink tile the sinks only, and its products are that much smaller
+  auto kv_keys = [&](int j) {
+    if (!WIN || j <= qt - first) return AT_BKV;
+    const int n = p.sinks - win_kv_tile(j, qt, first) * AT_BKV;
+    return n < AT_BKV ? (n + 15) & ~15 : AT_BKV;
+  };
   auto kv_row = [&](int j) { return (WIN ? win_kv_tile(j, qt, first) : j) * AT_BKV; };
   const CUtensorMap *tm_q, *tm_k, *tm_v;
   int k_head = kvh, v_head = kvh;
@@ -171,10 +176,11 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
       if (!mbar_wait_warp(bar(1 + st), (uint32_t)(j >> 1) & 1u, 13, abort_flag, p.status)) return false;
       tc_fence_after();
       const uint64_t dk = attn_desc_k<HD>(sbase + L::OFF_K + st * L::KV_BYTES);
+      const uint32_t idesc = WIN ? umma_idesc_bf16(AT_BQ, kv_keys(j), 0, 0) : idesc_s;
 #pragma unroll
       for (int t = 0; t < HD / 16; ++t) {
         const uint32_t off = (t >> 2) * 16384 + (t & 3) * 32;
-        umma_bf16_w(el, tmem + S_COL, umma_desc_advance(dq, off), umma_desc_advance(dk, off), idesc_s, t > 0);
+        umma_bf16_w(el, tmem + S_COL, umma_desc_advance(dq, off), umma_desc_advance(dk, off), idesc, t > 0);
       }
       umma_commit_w(el, bar(7));
       umma_commit_w(el, bar(11 + st));                              // K stage free
@@ -193,9 +199,12 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
       if (!mbar_wait_warp(bar(3 + st), (uint32_t)(j >> 1) & 1u, 15, abort_flag, p.status)) break;   // V landed
       tc_fence_after();
       const uint64_t dv = attn_desc_mn<HD>(sbase + L::OFF_V + st * L::KV_BYTES);   // MN-major: 16 kv rows per step
+      const int keys = kv_keys(j);
 #pragma unroll
-      for (int t = 0; t < AT_BKV / 16; ++t)                   // 16 kv = 8 columns of packed pairs per step
+      for (int t = 0; t < AT_BKV / 16; ++t) {                 // 16 kv = 8 columns of packed pairs per step
+        if (WIN && t * 16 >= keys) break;
         umma_bf16_ts_w(el, tmem + O_COL, tmem + P_COL + t * 8, umma_desc_advance(dv, t * attn_mn_step<HD>()), idesc_o, (j > 0) | (t > 0));
+      }
       umma_commit_w(el, bar(9));                                    // O updated, P free
       umma_commit_w(el, bar(5 + st));                               // V stage free
     }
@@ -351,16 +360,6 @@ static int launch_fwd(const AttnFwdMaps<WIN>& maps, const AttnFwdParams& p, cuda
   return launch_overlapped(attn_fwd_kernel<HD, WIN>, dim3(grid), dim3(AT_THREADS), L::TOTAL, st, 1, maps, p);
 }
 
-// The same over any [B, T, heads, hd] tensor; strides (batch, token, head) in elements, multiples of 8
-int make_bthd_map(CUtensorMap* map, const void* base, const long long* strides, int B, int T, int heads, int hd, int box_rows, int box_cols) {
-  if (!aligned16(base)) return -7;
-  for (int i = 0; i < 3; ++i) if (strides[i] <= 0 || strides[i] % 8 != 0 || strides[i] >= (1LL << 39)) return -7;
-  uint64_t dims[4] = {(uint64_t)hd, (uint64_t)heads, (uint64_t)T, (uint64_t)B};
-  uint64_t bytes[3] = {(uint64_t)strides[2] * 2, (uint64_t)strides[1] * 2, (uint64_t)strides[0] * 2};
-  uint32_t box[4] = {(uint32_t)box_cols, 1, (uint32_t)box_rows, 1};
-  return make_tmap_bf16(map, base, 4, dims, bytes, box);
-}
-
 }  // namespace tlm
 
 using namespace tlm;
@@ -409,10 +408,9 @@ TLM_API int tlm_attn_window_fwd(const void* q, const void* k, const void* v, con
   if (B < 0 || T < 0 || T > (1 << 30) || sinks < 0 || (long long)((T + AT_BQ - 1) / AT_BQ) * B * Hq > 0x7fffffffLL) return -6;
   if (B == 0 || T == 0) return 0;
   AttnFwdMaps<true> maps;
-  const int cols = hd == 32 ? 32 : 64;
-  int e = make_bthd_map(&maps.q, q, strides, B, T, Hq, hd, AT_BQ, cols);
-  if (!e) e = make_bthd_map(&maps.k, k, strides + 3, B, T, Hkv, hd, AT_BKV, cols);
-  if (!e) e = make_bthd_map(&maps.v, v, strides + 6, B, T, Hkv, hd, AT_BKV, cols);
+  int e = make_bthd_map(&maps.q, q, strides, B, T, Hq, hd, AT_BQ);
+  if (!e) e = make_bthd_map(&maps.k, k, strides + 3, B, T, Hkv, hd, AT_BKV);
+  if (!e) e = make_bthd_map(&maps.v, v, strides + 6, B, T, Hkv, hd, AT_BKV);
   if (e) return e;
   AttnFwdParams p{};
   p.o = (__nv_bfloat16*)o; p.lse = lse; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
