@@ -204,9 +204,10 @@ __global__ void attn_dq_convert_kernel(const float* dq_acc, __nv_bfloat16* __res
   }
 }
 
-// The window's conversion: rows of dQ (fp32 accumulator * scale -> bf16), with `rot` the transposed rotation on the way, then the
-// rows of dK and dV that the main kernel has not finished: with `rot` all of dK (bf16, in place), and the sink rows of dK and dV,
-// whose fp32 parts are added up slot by slot. An item is 8 low columns and their 8 partners (j + hd / 2) of a row.
+// The window's conversion: rows of dQ (fp32 accumulator * scale -> bf16), with a rotation its transposed form on the way, and what the
+// main kernel has not finished of dK and dV: with a rotation all rows of dK (bf16, in place), and the sink rows of both, whose fp32
+// parts are added up slot by slot. An item is 8 low columns and their 8 partners (j + hd / 2) of a row. The sums have blocks of
+// their own: beside the conversion, one item after the other, 28 slots of 16 rows took 15 us longer than everything else (T 32768).
 struct AttnWinFinish {
   const float* dq_acc;
   const float* part;                 // see AttnBwdParams
@@ -215,47 +216,92 @@ struct AttnWinFinish {
   const float *cosT, *sinT;
   int B, T, Hq, Hkv, hd;
   int sinks, slots, slot_rows;       // rows whose sums are in `part`, its slots and a slot's rows
-  int k_rows, v_rows;                // rows of a dK / dV head that are items: T with a rotation, the sinks, or none
+  int sum_blocks;                    // the first blocks of the grid
   float scale;
 };
+constexpr int WIN_FINISH_THREADS = 256;
 
-__global__ void __launch_bounds__(256)
+// kind: 0 dQ, 1 dK, 2 dV
+__device__ __forceinline__ void win_finish_item(const AttnWinFinish& p, int kind, __nv_bfloat16* dst, int t, int j, float* lo, float* hi) {
+  const int half = p.hd / 2;
+  if (p.cosT != nullptr && kind < 2) {
+    const float *c = p.cosT + (long long)t * p.hd + j, *sn = p.sinT + (long long)t * p.hd + j;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float a = lo[k], bb = hi[k];
+      lo[k] = a * c[k] + bb * sn[half + k];
+      hi[k] = bb * c[half + k] - a * sn[k];
+    }
+  }
+  *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
+  *reinterpret_cast<uint4*>(dst + half) = make_uint4(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]), pack_bf16(hi[4], hi[5]), pack_bf16(hi[6], hi[7]));
+}
+
+__global__ void __launch_bounds__(WIN_FINISH_THREADS)
 attn_window_finish_kernel(const AttnWinFinish p) {
   griddep_wait();
   griddep_launch();
-  const int half = p.hd / 2, vec_log = p.hd == 32 ? 1 : p.hd == 64 ? 2 : 3;          // hd / 16 items per row
-  const long long q_rows = (long long)p.B * p.Hq * p.T, k_all = (long long)p.B * p.Hkv * p.k_rows;
-  const long long total = (q_rows + k_all + (long long)p.B * p.Hkv * p.v_rows) << vec_log;
-  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+  const int half = p.hd / 2;
+  if ((int)blockIdx.x < p.sum_blocks) {
+    // a row of dV | dK: hd / 2 threads take 16 bytes of it each, as many groups of them as there are take slots in turn
+    __shared__ float4 sums[WIN_FINISH_THREADS];
+    const int vecs = p.hd / 2, groups = WIN_FINISH_THREADS / vecs, vec = threadIdx.x % vecs, group = threadIdx.x / vecs;
+    for (int r = blockIdx.x; r < p.B * p.Hkv * p.sinks; r += p.sum_blocks) {
+      const int bh = r / p.sinks, t = r - bh * p.sinks, b = bh / p.Hkv, h = bh - b * p.Hkv;
+      const float4* src = reinterpret_cast<const float4*>(p.part + ((long long)bh * p.slots * p.slot_rows + t) * (2 * p.hd)) + vec;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int n = group; n < p.slots; n += groups) {
+        const float4 x = src[(long long)n * p.slot_rows * (p.hd / 2)];
+        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+      }
+      sums[threadIdx.x] = a;
+      __syncthreads();
+      if (group == 0) {
+        for (int n = 1; n < groups; ++n) {
+          const float4 x = sums[n * vecs + vec];
+          a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+        }
+        sums[vec] = a;
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < p.hd / 8) {                 // hd / 16 items of dV, then of dK
+        const int kind = (int)threadIdx.x < p.hd / 16 ? 2 : 1, j = threadIdx.x % (p.hd / 16) * 8;
+        const float* row = reinterpret_cast<const float*>(sums) + (kind == 1 ? p.hd : 0) + j;
+        const float osc = kind == 1 ? p.scale : 1.f;
+        float lo[8], hi[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { lo[k] = row[k] * osc; hi[k] = row[half + k] * osc; }
+        __nv_bfloat16* dst = kind == 1 ? p.dk + b * p.dks[0] + t * p.dks[1] + h * p.dks[2] : p.dv + b * p.dvs[0] + t * p.dvs[1] + h * p.dvs[2];
+        win_finish_item(p, kind, dst + j, t, j, lo, hi);
+      }
+      __syncthreads();
+    }
+    return;
+  }
+  const int vec_log = p.hd == 32 ? 1 : p.hd == 64 ? 2 : 3;          // hd / 16 items per row
+  const int k_rows = p.cosT != nullptr ? p.T - p.sinks : 0;         // finished rows of dK, to be rotated
+  const long long q_rows = (long long)p.B * p.Hq * p.T, total = (q_rows + (long long)p.B * p.Hkv * k_rows) << vec_log;
+  const long long step = (long long)(gridDim.x - p.sum_blocks) * WIN_FINISH_THREADS;
+  for (long long i = (blockIdx.x - p.sum_blocks) * (long long)WIN_FINISH_THREADS + threadIdx.x; i < total; i += step) {
     const int j = (int)(i & ((1 << vec_log) - 1)) * 8;
     long long r = i >> vec_log;
-    const int kind = r < q_rows ? 0 : r < q_rows + k_all ? 1 : 2;               // dQ, dK, dV
-    if (kind > 0) r -= kind == 1 ? q_rows : q_rows + k_all;
-    const int rows = kind == 0 ? p.T : kind == 1 ? p.k_rows : p.v_rows, heads = kind == 0 ? p.Hq : p.Hkv;
-    const int bh = (int)(r / rows), t = (int)(r - (long long)bh * rows), b = bh / heads, h = bh - b * heads;
-    __nv_bfloat16* dst = kind == 0 ? p.dq + b * p.dqs[0] + t * p.dqs[1] + h * p.dqs[2]
-                       : kind == 1 ? p.dk + b * p.dks[0] + t * p.dks[1] + h * p.dks[2] : p.dv + b * p.dvs[0] + t * p.dvs[1] + h * p.dvs[2];
-    dst += j;
+    const int kind = r < q_rows ? 0 : 1;
+    if (kind == 1) r -= q_rows;
+    const int rows = kind == 0 ? p.T : k_rows, heads = kind == 0 ? p.Hq : p.Hkv;
+    const int bh = (int)(r / rows), t = (int)(r - (long long)bh * rows) + (kind == 0 ? 0 : p.sinks), b = bh / heads, h = bh - b * heads;
+    __nv_bfloat16* dst = (kind == 0 ? p.dq + b * p.dqs[0] + t * p.dqs[1] + h * p.dqs[2] : p.dk + b * p.dks[0] + t * p.dks[1] + h * p.dks[2]) + j;
     float lo[8], hi[8];
-    if (kind == 0 || (p.part != nullptr && t < p.sinks)) {
-      const float* src = kind == 0 ? p.dq_acc + ((long long)bh * p.T + t) * p.hd + j
-                                   : p.part + ((long long)bh * p.slots * p.slot_rows + t) * (2 * p.hd) + (kind == 1 ? p.hd : 0) + j;
-      const long long slot = (long long)p.slot_rows * 2 * p.hd;
-      const float osc = kind == 2 ? 1.f : p.scale;
+    if (kind == 0) {
+      const float* src = p.dq_acc + ((long long)bh * p.T + t) * p.hd + j;
 #pragma unroll
       for (int k = 0; k < 8; k += 4) {
         *reinterpret_cast<float4*>(lo + k) = *reinterpret_cast<const float4*>(src + k);
         *reinterpret_cast<float4*>(hi + k) = *reinterpret_cast<const float4*>(src + half + k);
       }
-      if (kind > 0)
-        for (int n = 1; n < p.slots; ++n) {
-          const float* s = src + n * slot;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) { lo[k] += s[k]; hi[k] += s[half + k]; }
-        }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) { lo[k] *= osc; hi[k] *= osc; }
-    } else {                                             // a finished row of dK, to be rotated
+      for (int k = 0; k < 8; ++k) { lo[k] *= p.scale; hi[k] *= p.scale; }
+    } else {
       const uint4 a = *reinterpret_cast<const uint4*>(dst), c = *reinterpret_cast<const uint4*>(dst + half);
       const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
@@ -264,17 +310,7 @@ attn_window_finish_kernel(const AttnWinFinish p) {
         lo[2 * k] = x.x; lo[2 * k + 1] = x.y; hi[2 * k] = y.x; hi[2 * k + 1] = y.y;
       }
     }
-    if (p.cosT != nullptr && kind < 2) {
-      const float *c = p.cosT + (long long)t * p.hd + j, *sn = p.sinT + (long long)t * p.hd + j;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float a = lo[k], bb = hi[k];
-        lo[k] = a * c[k] + bb * sn[half + k];
-        hi[k] = bb * c[half + k] - a * sn[k];
-      }
-    }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
-    *reinterpret_cast<uint4*>(dst + half) = make_uint4(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]), pack_bf16(hi[4], hi[5]), pack_bf16(hi[6], hi[7]));
+    win_finish_item(p, kind, dst, t, j, lo, hi);
   }
 }
 
@@ -1115,9 +1151,9 @@ TLM_API int tlm_attn_window_bwd(const void* q, const void* k, const void* v, con
   f.cosT = cosT; f.sinT = sinT; f.B = B; f.T = T; f.Hq = Hq; f.Hkv = Hkv; f.hd = hd; f.scale = scale; f.slots = 1 + p.far.chunks;
   f.slot_rows = p.sinks;                        // but only those of tiles with far query tiles are in use
   f.sinks = p.sinks < p.far.tiles * AB_TILE ? p.sinks : p.far.tiles * AB_TILE;
-  f.k_rows = cosT != nullptr ? T : f.sinks;
-  f.v_rows = f.sinks;
-  const long long items = ((long long)B * Hq * T + (long long)B * Hkv * (f.k_rows + f.v_rows)) * (hd / 16), blocks = (items + 255) / 256;
-  const int cb = (int)(blocks < num_sms() * 16 ? blocks : num_sms() * 16);
-  return launch_overlapped(attn_window_finish_kernel, dim3(cb), dim3(256), 0, st, 1, f);
+  const long long rows = (long long)B * Hkv * f.sinks, items = ((long long)B * Hq * T + (cosT != nullptr ? (long long)B * Hkv * (T - f.sinks) : 0)) * (hd / 16);
+  const long long blocks = (items + WIN_FINISH_THREADS - 1) / WIN_FINISH_THREADS;
+  f.sum_blocks = (int)(rows < num_sms() ? rows : num_sms());
+  const int cb = f.sum_blocks + (int)(blocks < num_sms() * 16 ? blocks : num_sms() * 16);
+  return launch_overlapped(attn_window_finish_kernel, dim3(cb), dim3(WIN_FINISH_THREADS), 0, st, 1, f);
 }
