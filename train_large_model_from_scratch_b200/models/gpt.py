@@ -228,14 +228,15 @@ class GPT(nn.Module):
         def form(block):                       # what the one call takes from the first block
             attn = block.attn
             return (attn.num_attention_heads, attn.num_key_value_heads, attn.head_dim, block.mlp._gate_up_weight.shape,
-                    attn.config.rope_theta, attn.config.rope_variant, block.ln_1.variance_epsilon)
+                    attn.config.rope_theta, attn.config.rope_variant, attn.config.rope_scaling, attn.config.rope_scaling_factor,
+                    attn.config.rope_original_length, block.ln_1.variance_epsilon)
 
         first = None
         for block in self.blocks:
             if type(block) is not Block or type(block.attn) is not Attention or type(block.mlp) is not MLP:
                 return False
             attn, mlp = block.attn, block.mlp
-            if (attn.training and attn.dropout > 0.0) or not F_ops.swiglu_mlp_fused_ok(attn.q_proj.weight, mlp._gate_up_weight) \
+            if (attn.training and attn.dropout > 0.0) or attn.window > 0 or attn.rotary_op or not F_ops.swiglu_mlp_fused_ok(attn.q_proj.weight, mlp._gate_up_weight) \
                     or not F_ops.qkv_project_fused_ok(attn.q_proj.weight, attn._qkv_weight, attn.head_dim, T):
                 return False
             for m in (block, attn, mlp, block.ln_1, block.ln_2):
@@ -286,13 +287,16 @@ class GPT(nn.Module):
 
     def get_exact_flops_per_fwd_bwd(self, batch_size: int, seq_len: int) -> float:
         """Corrected count per device: GQA projection sizes, causal attention
-        (half the score matrix), LM head included."""
+        (half the score matrix, or what the window leaves of it), LM head included."""
         c = self.config
         sp, ep = parallel_state.get_sp_world_size(), parallel_state.get_ep_world_size()
         B, T, D = batch_size, seq_len, c.hidden_size
         hd = D // c.num_attention_heads
         proj = 2 * B * T * D * (c.num_attention_heads * hd + 2 * c.num_key_value_heads * hd + D)
         attn = 4 * B * T * T * D / 2
+        if 0 < c.attn_window < T:                    # whole windows, the rows before the first one, and the sinks in front of them
+            W, late = c.attn_window, T - c.attn_window
+            attn = 4 * B * D * (W * W / 2 + late * (W + min(c.attn_sinks, late / 2)))
         if self.use_moe:
             ffn = 2 * B * T * D * c.num_experts + c.num_experts_per_tok * 6 * B * T * D * c.moe_intermediate_size
         else:

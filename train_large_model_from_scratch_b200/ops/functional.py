@@ -200,28 +200,34 @@ class _QKVAttention(torch.autograd.Function):
     fp32 accumulator, dK as it leaves tensor memory) instead of running a separate pass over the packed gradient."""
 
     @staticmethod
-    def forward(ctx, h, weight, cos, sin, cs, B, T, n_q, n_kv, hd):
+    def forward(ctx, h, weight, cos, sin, cs, B, T, n_q, n_kv, hd, window, sinks):
         Ht = n_q + 2 * n_kv
         qkv = torch.empty(B, T, Ht, hd, dtype=torch.bfloat16, device=h.device)
         import ctypes
         dst = (ctypes.c_void_p * 1)(qkv.data_ptr())
         native.gemm_heads(h, weight, False, dst, 1, B, T, T, Ht, 0, n_q, n_kv, n_q, max(n_kv, 1), hd, n_q + n_kv, cs,
                           tables=(cos, sin))
-        o, lse = native.flash_attn_fwd(qkv, n_q, n_kv, True)
+        if window > 0:
+            o, lse = native.window_attn_fwd_packed(qkv, n_q, n_kv, window, sinks)
+        else:
+            o, lse = native.flash_attn_fwd(qkv, n_q, n_kv, True)
         ctx.save_for_backward(h, qkv, o, lse, cos, sin)
-        ctx.weight, ctx.meta = weight, (n_q, n_kv)
+        ctx.weight, ctx.meta = weight, (n_q, n_kv, window, sinks)
         return o
 
     @staticmethod
     def backward(ctx, do):
         h, qkv, o, lse, cos, sin = ctx.saved_tensors
-        n_q, n_kv = ctx.meta
+        n_q, n_kv, window, sinks = ctx.meta
         w = ctx.weight
-        d = native.flash_attn_bwd(do.contiguous(), qkv, o, lse, n_q, n_kv, True, rope=(cos, sin))
+        if window > 0:
+            d = native.window_attn_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks, rope=(cos, sin))
+        else:
+            d = native.flash_attn_bwd(do.contiguous(), qkv, o, lse, n_q, n_kv, True, rope=(cos, sin))
         d2 = d.view(h.shape[0], -1)
         native.gemm_tn_accum(d2, h, _main_grad(w))
         dh = native.gemm_nn(d2, w) if ctx.needs_input_grad[0] else None
-        return dh, None, None, None, None, None, None, None, None, None
+        return dh, None, None, None, None, None, None, None, None, None, None, None
 
 
 def _table(t: torch.Tensor) -> torch.Tensor:
@@ -231,9 +237,10 @@ def _table(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def qkv_attention(h, weight, cos, sin, cs, B: int, T: int, n_q: int, n_kv: int, hd: int) -> torch.Tensor:
-    """CUDA only (same conditions as `qkv_project`): projection + RoPE + causal attention -> `[B, T, n_q, hd]`."""
-    return _QKVAttention.apply(h, weight, _table(cos), _table(sin), cs, B, T, n_q, n_kv, hd)
+def qkv_attention(h, weight, cos, sin, cs, B: int, T: int, n_q: int, n_kv: int, hd: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """CUDA only (same conditions as `qkv_project`): projection + RoPE + causal attention (over a window, see `attention_packed`)
+    -> `[B, T, n_q, hd]`."""
+    return _QKVAttention.apply(h, weight, _table(cos), _table(sin), cs, B, T, n_q, n_kv, hd, window, sinks)
 
 
 def qkv_project_fused_ok(h: torch.Tensor, weight: torch.Tensor | None, hd: int, T: int) -> bool:
@@ -351,8 +358,13 @@ def _check_window(x, n_q, n_kv, window, sinks, *others) -> None:
     if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
         raise ValueError(f"window {window}, sinks {sinks}: neither may be negative, and sinks need a window")
     _check_device(x, *others)
-    if _use_native(x) and x.shape[3] not in (32, 64, 128):
+    if not window_attention_ok(x):
         raise ValueError(f"head dim {x.shape[3]}: the window kernels have 32, 64 and 128")
+
+
+def window_attention_ok(x: torch.Tensor) -> bool:
+    """Whether `window_attention` has a kernel for heads like `x`'s (off the GPU it always has)."""
+    return not _use_native(x) or x.shape[3] in (32, 64, 128)
 
 
 class _Window(torch.autograd.Function):
@@ -482,19 +494,26 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, int
     return _Rotary.apply(x, turn) if x.requires_grad and torch.is_grad_enabled() else _turn(x, turn)
 
 
+def _anchors(x, weights):
+    """The weights as inputs of a node, only where the node would have no differentiable input without them: their gradients go to
+    `main_grad`, and a parameter that is an input ties the node to the stream on which the parameter was first used (a backward
+    pass cannot then be captured while an older graph of the same parameters lives)."""
+    return (None, None) if x.requires_grad or weights is None else weights
+
+
 class _QkNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, q_weight, k_weight, n_q, eps, turn):
+    def forward(ctx, x, _q_anchor, _k_anchor, weights, n_q, eps, turn):
         ctx.save_for_backward(x)
-        ctx.weights, ctx.n_q, ctx.eps, ctx.turn = (q_weight, k_weight), n_q, eps, turn
+        ctx.weights, ctx.n_q, ctx.eps, ctx.turn = weights, n_q, eps, turn
         turn.keep()
-        return _qk_norm_fwd(x, ctx.weights, n_q, eps, turn)
+        return _qk_norm_fwd(x, weights, n_q, eps, turn)
 
     @staticmethod
     def backward(ctx, dy):
         (x,) = ctx.saved_tensors
         ctx.turn.check()
-        return _qk_norm_bwd(dy.contiguous(), x, ctx.weights, ctx.n_q, ctx.eps, ctx.turn), None, None, None, None, None
+        return _qk_norm_bwd(dy.contiguous(), x, ctx.weights, ctx.n_q, ctx.eps, ctx.turn), None, None, None, None, None, None
 
 
 def _qk_norm_fwd(x, weights, n_q, eps, turn):
@@ -523,6 +542,13 @@ def _qk_norm_bwd(dy, x, weights, n_q, eps, turn, out=None):
     return dx if out is None else out.copy_(dx)
 
 
+def _check_norm(x, *weights) -> None:
+    for w in weights:
+        if tuple(w.shape) != (x.shape[3],) or w.dtype != x.dtype or not w.is_contiguous():
+            raise ValueError(f"weights have to be contiguous {x.dtype} [{x.shape[3]}], not {w.dtype} {tuple(w.shape)}")
+    _check_device(x, *weights)
+
+
 def qk_norm_rotary(x: torch.Tensor, n_q: int, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
                    inv_freq: torch.Tensor, eps: float = 1e-6, interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
     """`rotary` behind an RMS norm of every head of `x [B, T, H, hd]`: heads below `n_q` are scaled by `q_weight [hd]`, the others by
@@ -530,14 +556,68 @@ def qk_norm_rotary(x: torch.Tensor, n_q: int, q_weight: torch.Tensor, k_weight: 
     x, positions, inv_freq = _check_rotary(x, positions, inv_freq)
     if not 0 <= n_q <= x.shape[2]:
         raise ValueError(f"n_q {n_q} of {x.shape[2]} heads")
-    for w in (q_weight, k_weight):
-        if tuple(w.shape) != (x.shape[3],) or w.dtype != x.dtype or not w.is_contiguous():
-            raise ValueError(f"weights have to be contiguous {x.dtype} [{x.shape[3]}], not {w.dtype} {tuple(w.shape)}")
-    _check_device(x, q_weight, k_weight)
+    _check_norm(x, q_weight, k_weight)
     n_q, eps, turn = int(n_q), float(eps), _Turn(positions, inv_freq, interleaved, scale)
     if torch.is_grad_enabled() and (x.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
-        return _QkNormRotary.apply(x, q_weight, k_weight, n_q, eps, turn)
+        return _QkNormRotary.apply(x, *_anchors(x, (q_weight, k_weight)), (q_weight, k_weight), n_q, eps, turn)
     return _qk_norm_fwd(x, (q_weight, k_weight), n_q, eps, turn)
+
+
+class _RotaryAttention(torch.autograd.Function):
+    """Rotation (and norm) of the q and k heads of a packed projection, then attention over them and the v heads where they lie.
+    One node, so that the values are never copied beside the rotated heads, and the gradient of the rotation is taken in place in
+    the packed gradient."""
+
+    @staticmethod
+    def forward(ctx, qkv, _q_anchor, _k_anchor, weights, n_q, n_kv, eps, turn, window, sinks):
+        ctx.meta = (n_q, n_kv, eps, turn, window, sinks)
+        ctx.weights = weights
+        turn.keep()
+        raw, v = qkv[:, :, :n_q + n_kv], qkv[:, :, n_q + n_kv:]
+        qk = _turn(raw, turn) if ctx.weights is None else _qk_norm_fwd(raw, ctx.weights, n_q, eps, turn)
+        if _use_native(qkv):
+            o, lse = native.window_attn_fwd(qk[:, :, :n_q], qk[:, :, n_q:], v, window, sinks)
+        else:
+            o, lse, *_ = _attn_fwd_ref(qk[:, :, :n_q], qk[:, :, n_q:], v, True, window, sinks)
+            o = o.to(qkv.dtype).contiguous()
+        ctx.save_for_backward(qkv, qk, o, lse)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        qkv, qk, o, lse = ctx.saved_tensors
+        n_q, n_kv, eps, turn, window, sinks = ctx.meta
+        turn.check()
+        n_qk = n_q + n_kv
+        q, k, v = qk[:, :, :n_q], qk[:, :, n_q:], qkv[:, :, n_qk:]
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        if _use_native(qkv):
+            native.window_attn_bwd(do, q, k, v, o, lse, window, sinks, _heads_of(dqkv, n_q, n_kv))
+        else:
+            torch.cat(_attn_bwd_ref(do, q, k, v, o, True, window, sinks), dim=2, out=dqkv)
+        d = dqkv[:, :, :n_qk]
+        if ctx.weights is not None:
+            _qk_norm_bwd(d, qkv[:, :, :n_qk], ctx.weights, n_q, eps, turn, out=d)
+        elif _use_native(qkv):
+            native.qk_rotary(d, turn.positions, turn.inv_freq, interleaved=turn.interleaved, scale=turn.scale, inverse=True, out=d)
+        else:
+            d.copy_(_turn(d, turn, inverse=True))
+        return dqkv, None, None, None, None, None, None, None, None, None
+
+
+def rotary_attention(qkv: torch.Tensor, n_q: int, n_kv: int, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False,
+                     scale: float = 1.0, norm_weights=None, eps: float = 1e-6, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """`rotary` (with `norm_weights = (q_weight, k_weight)`: `qk_norm_rotary`) on the q and k heads of `qkv [B, T, n_q + 2 n_kv, hd]`
+    and `window_attention` over them -> `[B, T, n_q, hd]`."""
+    if qkv.dim() != 4 or qkv.shape[2] != n_q + 2 * n_kv:
+        raise ValueError(f"qkv has to be [B, T, {n_q + 2 * n_kv}, hd], not {tuple(qkv.shape)}")
+    qkv, positions, inv_freq = _check_rotary(qkv, positions, inv_freq)
+    _check_window(qkv, n_q, n_kv, window, sinks)
+    if norm_weights is not None:
+        norm_weights = tuple(norm_weights)
+        _check_norm(qkv, *norm_weights)
+    return _RotaryAttention.apply(qkv, *_anchors(qkv, norm_weights), norm_weights, n_q, n_kv, float(eps),
+                                  _Turn(positions, inv_freq, interleaved, scale), window, sinks)
 
 
 # --------------------------------------------------------------------------- SwiGLU

@@ -435,13 +435,14 @@ _LL3, _LL9 = _c.c_longlong * 3, _c.c_longlong * 9
 
 
 def qk_rotary(x, positions, inv_freq, weights=None, n_q: int = 0, eps: float = 0.0, interleaved: bool = False, scale: float = 1.0,
-              inverse: bool = False) -> torch.Tensor:
+              inverse: bool = False, out=None) -> torch.Tensor:
     """`x [B, T, H, hd]` bf16 (rows contiguous) rotated by `positions` (int64, `[T]` or `[B, T]`) and `inv_freq` (float64), with
-    `weights = (q, k)` behind an RMS norm of every head (`csrc/qk_rotary.cu`). `inverse`: the transposed rotation, without norm."""
+    `weights = (q, k)` behind an RMS norm of every head (`csrc/qk_rotary.cu`). `inverse`: the transposed rotation, without norm.
+    `out`: where it goes, may be `x` itself."""
     B, T, H, hd = x.shape
-    y = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=x.device)
+    y = out if out is not None else torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=x.device)
     wq, wk = (w.data_ptr() for w in weights) if weights is not None else (None, None)
-    _check(lib().tlm_qk_rotary(x.data_ptr(), _LL3(*x.stride()[:3]), y.data_ptr(), _LL3(T * H * hd, H * hd, hd), positions.data_ptr(),
+    _check(lib().tlm_qk_rotary(x.data_ptr(), _LL3(*x.stride()[:3]), y.data_ptr(), _LL3(*y.stride()[:3]), positions.data_ptr(),
                                T if positions.dim() > 1 else 0, inv_freq.data_ptr(), inv_freq.shape[0], wq, wk, B, T, H, n_q, hd, eps,
                                scale, interleaved, inverse, _stream()), "qk_rotary")
     return y

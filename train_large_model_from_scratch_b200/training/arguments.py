@@ -88,6 +88,14 @@ _FLAG_TABLE: list[tuple[str, list[tuple[str, dict]]]] = [
         ("--moe_aux_loss_coef", dict(type=float, default=0.0, help="(added) load-balance loss weight")),
         ("--moe_capacity_factor", dict(type=float, default=0.0, help="(added) 0 = dropless")),
         ("--rope_variant", dict(type=str, default="reference", choices=["reference", "standard"], help="(added)")),
+        ("--attn_window", dict(type=int, default=0, help="(added) keys a query sees, itself included; 0 = all")),
+        ("--attn_sinks", dict(type=int, default=0, help="(added) first keys that stay visible besides the window")),
+        ("--qk_norm", dict(action=_S, help="(added) RMS norm of every query and key head before the rotation")),
+        ("--rope_layout", dict(type=str, default="half", choices=["half", "interleaved"], help="(added) which elements of a head turn together")),
+        ("--rope_fraction", dict(type=float, default=1.0, help="(added) part of the head that turns")),
+        ("--rope_scaling", dict(type=str, default="none", choices=["none", "linear", "ntk", "yarn"], help="(added) frequencies for contexts longer than the trained ones")),
+        ("--rope_scaling_factor", dict(type=float, default=1.0, help="(added)")),
+        ("--rope_original_length", dict(type=int, default=4096, help="(added) yarn: the length the unscaled frequencies were trained on")),
     ]),
 ]
 

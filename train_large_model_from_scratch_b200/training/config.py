@@ -12,7 +12,8 @@ Differences, all deliberate:
     crashes because it is missing, `training/trainer.py:398`).
   * Extra optional knobs with reference-parity defaults: `moe_aux_loss_coef`
     (0.0 = no auxiliary loss, as in the reference), `moe_capacity_factor`
-    (0.0 = dropless), `rope_variant` ("reference"), `grad_wire_dtype`,
+    (0.0 = dropless), `rope_variant` ("reference"), the attention window, norms
+    of queries and keys and the rotary forms (all off), `grad_wire_dtype`,
     `heartbeat_timeout_s` (0 = off), `dist_timeout_s`.
 """
 from __future__ import annotations
@@ -127,6 +128,14 @@ class ModelConfig:
     moe_capacity_factor: float = 0.0
     rope_variant: str = "reference"     # "reference" | "standard"
     rope_theta: float = 10000.0
+    attn_window: int = 0                # keys a query sees, itself included; 0: all
+    attn_sinks: int = 0                 # first keys that stay visible besides the window
+    qk_norm: bool = False               # RMS norm of every query and key head before the rotation
+    rope_layout: str = "half"           # "half" | "interleaved": which elements of a head turn together
+    rope_fraction: float = 1.0          # part of the head that turns
+    rope_scaling: str = "none"          # "none" | "linear" | "ntk" | "yarn"
+    rope_scaling_factor: float = 1.0
+    rope_original_length: int = 4096    # "yarn": the length that the unscaled frequencies were trained on
 
     def as_dict(self) -> dict[str, Any]:
         return asdict(self)
@@ -134,6 +143,32 @@ class ModelConfig:
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_attention_heads
+
+    @property
+    def rotary_dim(self) -> int:
+        """Elements of a head that turn with the position."""
+        return round(self.head_dim * self.rope_fraction)
+
+    @property
+    def rotary_op(self) -> bool:
+        """Whether the rotation is more than the projection's epilogue can do (normed heads, interleaved pairs, part of a head)."""
+        return self.qk_norm or self.rope_layout != "half" or self.rope_fraction != 1.0
+
+    def check_attention(self) -> None:
+        if self.attn_window < 0 or self.attn_sinks < 0 or (self.attn_sinks > 0 and self.attn_window == 0):
+            raise ValueError("attn_window and attn_sinks may not be negative, and attn_sinks needs an attn_window.")
+        if self.rope_layout not in ("half", "interleaved"):
+            raise ValueError(f"Unknown rope_layout: {self.rope_layout}")
+        if self.rope_scaling not in ("none", "linear", "ntk", "yarn"):
+            raise ValueError(f"Unknown rope_scaling: {self.rope_scaling}")
+        if self.rope_scaling_factor < 1.0 or self.rope_original_length < 1:
+            raise ValueError("rope_scaling_factor must be at least 1, rope_original_length positive.")
+        if not 0.0 < self.rope_fraction <= 1.0 or abs(self.head_dim * self.rope_fraction - self.rotary_dim) > 1e-6 or self.rotary_dim % 2:
+            raise ValueError(f"rope_fraction {self.rope_fraction} of a head of {self.head_dim} must be an even number of elements.")
+        if (self.rotary_op or self.rope_scaling != "none") and self.rope_variant != "standard":
+            raise ValueError("qk_norm, rope_layout, rope_fraction and rope_scaling need rope_variant 'standard'.")
+        if self.dropout > 0.0 and (self.attn_window > 0 or self.rotary_op):
+            raise ValueError("attention dropout runs on the library kernel, which has no attn_window, qk_norm, rope_layout or rope_fraction.")
 
 
 @dataclass(frozen=True)
@@ -206,5 +241,6 @@ def validate_static(cfg: Config) -> None:
         raise ValueError("num_experts_per_tok must be <= num_experts.")
     if m.rope_variant not in ("reference", "standard"):
         raise ValueError(f"Unknown rope_variant: {m.rope_variant}")
+    m.check_attention()
     if cfg.parallel.grad_wire_dtype not in ("bf16", "fp32"):
         raise ValueError(f"Unknown grad_wire_dtype: {cfg.parallel.grad_wire_dtype}")
