@@ -56,15 +56,19 @@ __device__ __forceinline__ uint32_t first_bits(int n, int w) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
-template <int HD>
+// ALIAS: P takes the place of S in tensor memory and K and V have one stage each, so that two blocks share an SM at head dim 128 too.
+// The next scores then wait for P V, a longer way from tile to tile, but the other block's exponentials run beside it: B 2, T 4096,
+// 16 / 4 heads of 128, window 2048 134 us with one block an SM.
+template <int HD, bool ALIAS = false>
 struct AttnFwdSmem {
+  static constexpr int STAGES = ALIAS ? 1 : AT_KV_STAGES;
   static constexpr int KB = HD == 128 ? 2 : 1;         // blocks along hd (64 wide; HD 32: one of 32)
   static constexpr int Q_BYTES = AT_BQ * HD * 2;
   static constexpr int KV_BYTES = AT_BKV * HD * 2;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + Q_BYTES;
-  static constexpr int OFF_V = OFF_K + AT_KV_STAGES * KV_BYTES;
-  static constexpr int OFF_BAR = OFF_V + AT_KV_STAGES * KV_BYTES;
+  static constexpr int OFF_V = OFF_K + STAGES * KV_BYTES;
+  static constexpr int OFF_BAR = OFF_V + STAGES * KV_BYTES;
   static constexpr int TOTAL = OFF_BAR + 256;          // + barriers; 2 CTAs (hd 64) must fit in 228 KB
 };
 
@@ -76,14 +80,18 @@ struct AttnFwdSmem {
 constexpr float RESCALE_LOG2 = 8.0f;
 
 template <int HD, bool WIN = false>
-__global__ void __launch_bounds__(AT_THREADS, HD <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(AT_THREADS, HD <= 64 || WIN ? 2 : 1)
 attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams p) {
-  using L = AttnFwdSmem<HD>;
+  constexpr bool ALIAS = WIN && HD == 128;
+  using L = AttnFwdSmem<HD, ALIAS>;
   constexpr int KB = L::KB;
   // tensor-memory columns: S (128 fp32), O (HD fp32) and the probabilities as packed bf16 pairs (64 columns),
   // which the P V MMA reads as its A operand straight from tensor memory (P never touches shared memory)
-  constexpr uint32_t S_COL = 0, O_COL = 128, P_COL = 128 + HD;
-  constexpr uint32_t TMEM_COLS = HD == 128 ? 512 : 256;
+  constexpr uint32_t S_COL = 0, O_COL = 128, P_COL = ALIAS ? S_COL : 128 + HD;
+  constexpr uint32_t TMEM_COLS = HD == 128 && !ALIAS ? 512 : 256;
+  // stage of step j's K and V, and how often it has been used before
+  auto stage = [](int j) { return ALIAS ? 0 : j & 1; };
+  auto uses = [](int j) { return (uint32_t)(ALIAS ? j : j >> 1); };
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
   uint8_t* sal = smem_raw;
@@ -142,8 +150,8 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) tma_load_4d(sbase + L::OFF_Q + kb * 16384, tm_q, bar(0), kb * 64, h, q0, b);
       auto load_k = [&](int j) -> bool {
-        const int st = j & 1;
-        if (!mbar_wait(bar(11 + st), ((uint32_t)(j >> 1) & 1u) ^ 1u, 11, abort_flag, p.status)) return false;
+        const int st = stage(j);
+        if (!mbar_wait(bar(11 + st), (uses(j) & 1u) ^ 1u, 11, abort_flag, p.status)) return false;
         mbar_expect_tx(bar(1 + st), L::KV_BYTES);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -152,13 +160,14 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
       };
       bool ok = load_k(0);
       for (int j = 0; j < n_kv && ok; ++j) {
-        const int st = j & 1;
-        if (j + 1 < n_kv && !load_k(j + 1)) break;
-        if (!mbar_wait(bar(5 + st), ((uint32_t)(j >> 1) & 1u) ^ 1u, 20, abort_flag, p.status)) break;
+        const int st = stage(j);
+        if (!ALIAS && j + 1 < n_kv && !load_k(j + 1)) break;
+        if (!mbar_wait(bar(5 + st), (uses(j) & 1u) ^ 1u, 20, abort_flag, p.status)) break;
         mbar_expect_tx(bar(3 + st), L::KV_BYTES);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
           tma_load_4d(sbase + L::OFF_V + st * L::KV_BYTES + kb * 16384, tm_v, bar(3 + st), kb * 64, v_head, kv_row(j), b);
+        if (ALIAS && j + 1 < n_kv && !load_k(j + 1)) break;
       }
     }
   } else if (warp == 1) {
@@ -172,8 +181,8 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
     constexpr uint32_t idesc_o = umma_idesc_bf16(AT_BQ, HD, 0, 1);
     const uint64_t dq = attn_desc_k<HD>(sbase + L::OFF_Q);
     auto issue_s = [&](int j) -> bool {
-      const int st = j & 1;
-      if (!mbar_wait_warp(bar(1 + st), (uint32_t)(j >> 1) & 1u, 13, abort_flag, p.status)) return false;
+      const int st = stage(j);
+      if (!mbar_wait_warp(bar(1 + st), uses(j) & 1u, 13, abort_flag, p.status)) return false;
       tc_fence_after();
       const uint64_t dk = attn_desc_k<HD>(sbase + L::OFF_K + st * L::KV_BYTES);
       const uint32_t idesc = WIN ? umma_idesc_bf16(AT_BQ, kv_keys(j), 0, 0) : idesc_s;
@@ -189,14 +198,14 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
     bool ok = mbar_wait_warp(bar(0), 0, 12, abort_flag, p.status);
     if (ok) ok = issue_s(0);
     for (int j = 0; j < n_kv && ok; ++j) {
-      const int st = j & 1;
+      const int st = stage(j);
       const uint32_t par = (uint32_t)j & 1u;
-      if (j + 1 < n_kv) {                                     // S of the next tile overlaps this tile's softmax
+      if (!ALIAS && j + 1 < n_kv) {                                     // S of the next tile overlaps this tile's softmax
         if (!mbar_wait_warp(bar(10), par, 18, abort_flag, p.status)) break;
         if (!issue_s(j + 1)) break;
       }
       if (!mbar_wait_warp(bar(8), par, 14, abort_flag, p.status)) break;                        // P written
-      if (!mbar_wait_warp(bar(3 + st), (uint32_t)(j >> 1) & 1u, 15, abort_flag, p.status)) break;   // V landed
+      if (!mbar_wait_warp(bar(3 + st), uses(j) & 1u, 15, abort_flag, p.status)) break;   // V landed
       tc_fence_after();
       const uint64_t dv = attn_desc_mn<HD>(sbase + L::OFF_V + st * L::KV_BYTES);   // MN-major: 16 kv rows per step
       const int keys = kv_keys(j);
@@ -207,6 +216,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
       }
       umma_commit_w(el, bar(9));                                    // O updated, P free
       umma_commit_w(el, bar(5 + st));                               // V stage free
+      if (ALIAS && j + 1 < n_kv && !issue_s(j + 1)) break;          // behind P V, which reads what these scores replace
     }
     griddep_launch();
   } else {
@@ -349,7 +359,7 @@ int make_qkv_map(CUtensorMap* map, const void* base, int B, int T, int heads, in
 
 template <int HD, bool WIN = false>
 static int launch_fwd(const AttnFwdMaps<WIN>& maps, const AttnFwdParams& p, cudaStream_t st) {
-  using L = AttnFwdSmem<HD>;
+  using L = AttnFwdSmem<HD, WIN && HD == 128>;
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
