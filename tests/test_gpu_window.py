@@ -166,6 +166,23 @@ def test_hidden_keys_may_hold_anything_finite():
         assert torch.equal(got[0][:, rows], base[0][:, rows])
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_a_key_of_nan_reaches_the_rows_that_see_it(d):
+    """... and no others: a hidden score is hidden whatever it is."""
+    n_q, n_kv, window, sinks = 2, 1, 40, 3
+    qkv, do = _inputs(1, 400, n_q, n_kv, d, seed=10)
+    base = _run_packed(qkv, do, n_q, n_kv, window, sinks)[0]
+    for at in (1, 130, 131, 135, 139, 250, 399):
+        bad = qkv.clone()
+        bad[:, at, n_q] = float("nan")
+        from train_large_model_from_scratch_b200.ops import functional as F_ops
+        with torch.no_grad():
+            o = F_ops.attention_packed(bad, n_q, n_kv, window=window, sinks=sinks)
+        row = torch.arange(400, device="cuda")
+        sees = (row >= at) & ((row - at < window) | (at < sinks))
+        assert torch.isnan(o[:, sees]).all() and torch.equal(o[:, ~sees], base[:, ~sees]), at
+
+
 def test_same_bits_again_and_in_a_graph():
     """o, dk and dv do not depend on the order in which blocks run (dq is reduced in hardware order); a captured call replays on
     new inputs, beside another captured call and eager ones on another stream."""

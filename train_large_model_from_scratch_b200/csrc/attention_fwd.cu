@@ -79,6 +79,22 @@ struct AttnFwdSmem {
 // is used for P and for the final normalisation.
 constexpr float RESCALE_LOG2 = 8.0f;
 
+// 2^x for x <= 127 on the FMA pipe: x = n + f with n the nearest integer (the sum with 1.5 * 2^23 + 127 leaves n + 127 in the low bits), a
+// polynomial of degree 3 for 2^f on [-1/2, 1/2] (minimax, off by 7.5e-5, a fiftieth of half a bf16 step), times 2^n.
+// Below -126, -infinity included, that is 0.99993 * 2^-126; less 2^-126 it is nearer to zero than to any bf16, and so a hidden key's
+// probability is. NaN stays NaN.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));      // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  const float2 magic = make_float2(12583039.f, 12583039.f);
+  const float2 t = fadd2(x, magic), f = fadd2(x, fadd2(magic, make_float2(-t.x, -t.y)));
+  float2 q = ffma2(f, make_float2(0.05517166f, 0.05517166f), make_float2(0.24261112f, 0.24261112f));
+  q = ffma2(f, q, make_float2(0.69326099f, 0.69326099f));
+  q = ffma2(f, q, make_float2(0.99992807f, 0.99992807f));
+  const float2 two_n = make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23));
+  return ffma2(q, two_n, make_float2(-1.17549435e-38f, -1.17549435e-38f));
+}
+
 template <int HD, bool WIN = false>
 __global__ void __launch_bounds__(AT_THREADS, HD <= 64 || WIN ? 2 : 1)
 attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams p) {
@@ -273,13 +289,17 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
       else if (grow) { alpha = ex2_approx((m_ref - mx) * p.scale_log2); m_ref = mx; }
       const float neg_m = -m_ref * p.scale_log2;
       // ---- probabilities as packed bf16 pairs, still in registers (they take the place of the S row)
+      // WIN takes every seventh pair of probabilities this way: the exponential unit takes 1024 cycles for a tile, two warps share it, and the
+      // rest of a warp's way from tile to tile is too short to hide that (at best 58 % of its cycles were in use). In us, no pair / every
+      // eighth / seventh / fifth: B 8, T 4096, 16 / 8 heads of 64, window 1024 248 / 230 / 228 / 231; 32 / 4 of 32, window 512 331 / 316 / 313 /
+      // 317; B 2, 16 / 4 of 128, window 2048 120 / 118 / 116 / 118.
       float2 l2 = make_float2(0.f, 0.f);
       const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(neg_m, neg_m);
       uint32_t pk[AT_BKV / 2];
 #pragma unroll
       for (int i = 0; i < AT_BKV; i += 2) {
         const float2 x = ffma2(make_float2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), sc2, nm2);
-        float2 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+        float2 pp = WIN && (i >> 1) % 7 == 6 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
         if (diag) { if (i > row) pp.x = 0.f; if (i + 1 > row) pp.y = 0.f; }
         l2 = fadd2(l2, pp);
         pk[i >> 1] = pack_bf16(pp.x, pp.y);
