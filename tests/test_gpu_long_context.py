@@ -206,3 +206,36 @@ def test_captured_beside_an_eager_graph_of_the_same_parameters(which):
     assert torch.equal(got[0], want[0])
     for a, b in zip(got[1:], want[1:]):
         assert ((a.double() - b.double()).norm() <= 2 * H * b.double().norm()).item()
+
+
+def test_forward_at_another_length_between_recorded_steps():
+    """Scoring a prompt of another length between two steps replaces the positions and frequencies that the model caches; the recorded
+    step goes on reading the ones it was recorded with."""
+    import tempfile
+    from train_large_model_from_scratch_b200.training import Trainer
+    from train_large_model_from_scratch_b200.training.config import (CheckpointConfig, Config, DataConfig, LoggingConfig, ModelConfig,
+                                                                     OptimConfig, ParallelConfig, SeedConfig, TrainingConfig)
+    data = torch.randint(0, 2048, (2, 257), generator=torch.Generator().manual_seed(8)).cuda()
+    batch = [{"input_ids": data[:, :-1].contiguous(), "labels": data[:, 1:].contiguous()}]
+    runs = []
+    for other_lengths in (False, True):
+        tr = Trainer(Config(
+            logging=LoggingConfig(exp_name="t", log_dir=tempfile.mkdtemp(prefix="tlm_gpu_")), seed=SeedConfig(),
+            data=DataConfig(use_mock_data=True, mock_data_num_samples=2),
+            train=TrainingConfig(total_batch_size=512, batch_size=2, seq_len=256, max_steps=100, max_epochs=None, debug=True).with_derived(),
+            optim=OptimConfig(max_lr=6e-4, min_lr=6e-5, warmup_steps=10), ckpt=CheckpointConfig(), parallel=ParallelConfig(),
+            model=ModelConfig(num_layer=2, hidden_size=256, num_attention_heads=4, num_key_value_heads=2, intermediate_size=512, vocab_size=2048,
+                              block_size=512, rope_variant="standard", rope_layout="interleaved", qk_norm=True, attn_window=70, attn_sinks=2)))
+        run = []
+        for step in range(7):
+            run.append(float(tr.train_step(step, batches=batch)["loss"]))
+            if other_lengths and step >= 3:
+                logits, _, _ = tr.raw_model(data[:, :100])
+                del logits
+                junk = [torch.full((256,), 12345, device="cuda") for _ in range(64)] + \
+                       [torch.full((n,), 3.0, device="cuda", dtype=torch.float64) for n in (32, 256) for _ in range(64)]
+                del junk
+        assert tr._graph is not None
+        runs.append(run)
+    for a, b in zip(*runs):
+        assert math.isfinite(a) and abs(a - b) < 5e-3 * a, runs

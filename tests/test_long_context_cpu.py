@@ -237,3 +237,16 @@ def test_ranks_of_a_sequence_group_agree():
                 assert abs(a[key][step] - b[key][step]) <= 2e-4 * max(1.0, abs(a[key][step])), (key, step)
     finally:
         shutil.rmtree(tmp, ignore_errors=True)
+
+
+def test_a_step_that_exchanges_heads_through_the_library_is_not_recorded():
+    from types import SimpleNamespace
+    from train_large_model_from_scratch_b200.training import Trainer
+
+    def eligible(sp, **model):
+        cfg = build_config(parse_args(["--rope_variant", "standard"] + [f for k, v in model.items() for f in (f"--{k}", str(v))]))
+        return Trainer._graph_eligible(SimpleNamespace(_graph_disabled=False, use_cuda=True, config=cfg, world_size=2, _symm=True, sp_world_size=sp,
+                                                       _compute_dtype=lambda p: torch.bfloat16))
+
+    assert eligible(2) and eligible(1, attn_window=8) and eligible(1, rope_fraction=0.5)
+    assert not eligible(2, attn_window=8) and not eligible(2, rope_fraction=0.5)

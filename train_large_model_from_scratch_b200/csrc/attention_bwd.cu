@@ -984,12 +984,8 @@ template <int HD, bool SCATTER, bool SPLIT = false, bool WIN = false>
 static int launch_bwd(const AttnBwdMaps<WIN>& maps, const AttnBwdParams& p, cudaStream_t st) {
   constexpr int smem = AttnBwdCfg<HD>::TOTAL;
   auto kern = attn_bwd_kernel<HD, SCATTER, SPLIT, WIN>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemConfigured configured;
+  if (const int e = configured.set(kern, smem)) return e;
   const int grid = ((p.T + AB_TILE - 1) / AB_TILE + (WIN ? p.far.tiles * p.far.chunks : 0)) * p.B * p.Hkv;
   return launch_overlapped(kern, dim3((unsigned)(grid * (SPLIT ? p.split : 1))), dim3(AB_THREADS), smem, st, SPLIT ? p.split : 1, maps, p);
 }
@@ -1092,7 +1088,7 @@ TLM_API int tlm_attn_bwd_scatter(const void* qkv, const void* o, const void* dou
 
 // Floats of `part` that tlm_attn_window_bwd needs (0: none).
 TLM_API long long tlm_attn_window_part_floats(int B, int T, int Hkv, int hd, int window, int sinks) {
-  if (T <= 0 || T > (1 << 30)) return 0;
+  if (T <= 0 || T > (1 << 29)) return 0;
   const int S = sinks < T ? sinks : T;
   const WinFar f = win_far(T, window > 0 && window < T ? window : T, S);
   return f.chunks > 0 ? (long long)B * Hkv * (1 + f.chunks) * S * 2 * hd : 0;
@@ -1108,7 +1104,7 @@ TLM_API int tlm_attn_window_bwd(const void* q, const void* k, const void* v, con
   if (hd != 32 && hd != 64 && hd != 128) return -4;
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return -5;
   if ((size_t)Hq * (DELTA_T + 1) * 4 > 48 * 1024) return -6;
-  if (B < 0 || T < 0 || T > (1 << 30) || sinks < 0 || (cosT == nullptr) != (sinT == nullptr)) return -6;
+  if (B < 0 || T < 0 || T > (1 << 29) || sinks < 0 || (cosT == nullptr) != (sinT == nullptr)) return -6;
   if (B == 0 || T == 0) return 0;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return -7;
   for (int i = 0; i < 9; ++i) if (out_strides[i] % 8 != 0) return -7;

@@ -380,12 +380,8 @@ int make_qkv_map(CUtensorMap* map, const void* base, int B, int T, int heads, in
 template <int HD, bool WIN = false>
 static int launch_fwd(const AttnFwdMaps<WIN>& maps, const AttnFwdParams& p, cudaStream_t st) {
   using L = AttnFwdSmem<HD, WIN && HD == 128>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemConfigured configured;
+  if (const int e = configured.set(attn_fwd_kernel<HD, WIN>, L::TOTAL)) return e;
   const int grid = ((p.T + AT_BQ - 1) / AT_BQ) * p.B * p.Hq;
   return launch_overlapped(attn_fwd_kernel<HD, WIN>, dim3(grid), dim3(AT_THREADS), L::TOTAL, st, 1, maps, p);
 }
@@ -435,7 +431,7 @@ TLM_API int tlm_attn_window_fwd(const void* q, const void* k, const void* v, con
                                 int Hq, int Hkv, int hd, float scale, int window, int sinks, cudaStream_t st) {
   if (hd != 32 && hd != 64 && hd != 128) return -4;
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return -5;
-  if (B < 0 || T < 0 || T > (1 << 30) || sinks < 0 || (long long)((T + AT_BQ - 1) / AT_BQ) * B * Hq > 0x7fffffffLL) return -6;
+  if (B < 0 || T < 0 || T > (1 << 29) || sinks < 0 || (long long)((T + AT_BQ - 1) / AT_BQ) * B * Hq > 0x7fffffffLL) return -6;
   if (B == 0 || T == 0) return 0;
   AttnFwdMaps<true> maps;
   int e = make_bthd_map(&maps.q, q, strides, B, T, Hq, hd, AT_BQ);

@@ -73,6 +73,22 @@ inline int launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, size_t s
 }
 #endif
 
+#ifdef __CUDACC__
+// Dynamic shared memory of a kernel, asked for once on every device.
+struct SmemConfigured {
+  unsigned long long devices = 0;
+  template <typename K>
+  int set(K kern, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (devices >> dev & 1ull))) return (int)e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) devices |= 1ull << dev;
+    return (int)e;
+  }
+};
+#endif
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 inline int launch_status() {

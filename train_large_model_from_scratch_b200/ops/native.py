@@ -454,6 +454,8 @@ def qk_norm_rotary_bwd(dy, x, positions, inv_freq, weights, grads, n_q: int, eps
     B, T, H, hd = x.shape
     if out is None:
         out = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=x.device)
+    for g in grads:
+        assert g.dtype == torch.float32 and g.shape == (hd,) and g.is_contiguous() and g.device == x.device
     work = torch.empty(lib().tlm_qk_norm_work_floats(hd), dtype=torch.float32, device=x.device)
     _check(lib().tlm_qk_norm_rotary_bwd(x.data_ptr(), _LL3(*x.stride()[:3]), dy.data_ptr(), _LL3(*dy.stride()[:3]), out.data_ptr(),
                                         _LL3(*out.stride()[:3]), positions.data_ptr(), T if positions.dim() > 1 else 0,

@@ -384,6 +384,8 @@ class Trainer:
             return False
         if self.world_size > 1 and not getattr(self, "_symm", False):
             return False
+        if self.sp_world_size > 1 and (self.config.model.attn_window > 0 or self.config.model.rotary_op):
+            return False                                    # these exchange heads through the library
         return not self.config.train.use_profiler
 
     def _device_step(self):
@@ -467,7 +469,7 @@ class Trainer:
                 self._graph = graph
                 # the recording reads the rotation tables at their addresses: a forward at another length replaces the
                 # modules' cached tables, which must not free these
-                self._graph_tables = [(b.attn._rope_cache, b.attn._rope_cache_fp16, b.attn._rope_cache_full)
+                self._graph_tables = [(b.attn._rope_cache, b.attn._rope_cache_fp16, b.attn._rope_cache_full, b.attn._turn_cache)
                                       for b in self.raw_model.blocks]
             self._graph.replay()
             native.add_launch_count(self._graph_launches)
