@@ -135,15 +135,15 @@ def test_without_a_window_it_is_the_causal_operator():
 @pytest.mark.parametrize("d,variant", [(32, "standard"), (64, "reference"), (128, "standard")])
 def test_transposed_rotation_on_the_way_out(d, variant):
     """`rope`: dQ and dK leave as gradients of the un-rotated heads, the sink rows of dK among them."""
-    from train_large_model_from_scratch_b200.ops import native, oracle
+    from train_large_model_from_scratch_b200.ops import attention_cuda, native, oracle
     T, n_q, n_kv = 1500, 2, 1
     qkv, do = _inputs(1, T, n_q, n_kv, d, seed=5)
     q, k, v = qkv.split([n_q, n_kv, n_kv], dim=2)
     cos, sin = oracle.rope_tables(torch.arange(T, device="cuda"), d, 10000.0, variant)
-    o, lse = native.window_attn_fwd(q, k, v, 100, 5)
+    o, lse = attention_cuda.window_fwd(q, k, v, 100, 5)
     plain, turned = ([torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v)] for _ in range(2))
-    native.window_attn_bwd(do, q, k, v, o, lse, 100, 5, plain)
-    native.window_attn_bwd(do, q, k, v, o, lse, 100, 5, turned, rope=(cos, sin))
+    attention_cuda.window_bwd(do, q, k, v, o, lse, 100, 5, plain)
+    attention_cuda.window_bwd(do, q, k, v, o, lse, 100, 5, turned, rope=(cos, sin))
     native.raise_on_device_status()
     assert torch.equal(plain[2], turned[2])
     for a, b in zip(plain[:2], turned[:2]):
@@ -236,8 +236,8 @@ def test_first_call_of_a_thread():
     x = torch.zeros(1, 77, 4, 64, device="cuda", dtype=torch.bfloat16)
 
     def call():
-        from train_large_model_from_scratch_b200.ops import native
-        got.append(native.window_attn_fwd(x[:, :, :2], x[:, :, 2:3], x[:, :, 3:], 11, 1)[0])
+        from train_large_model_from_scratch_b200.ops import attention_cuda
+        got.append(attention_cuda.window_fwd(x[:, :, :2], x[:, :, 2:3], x[:, :, 3:], 11, 1)[0])
 
     t = threading.Thread(target=call)
     t.start()

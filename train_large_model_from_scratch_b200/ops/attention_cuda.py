@@ -6,6 +6,7 @@ ATen (a library call, like a cuBLAS GEMM).
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -142,6 +143,11 @@ def _window_fwd(q: int, k: int, v: int, strides, B: int, T: int, n_q: int, n_kv:
     return o, lse
 
 
+@functools.lru_cache(maxsize=1024)
+def _part_floats(B: int, T: int, n_kv: int, hd: int, window: int, sinks: int) -> int:
+    return native.lib().tlm_attn_window_part_floats(B, T, n_kv, hd, window, sinks)
+
+
 def _window_bwd(do, q: int, k: int, v: int, strides, o, lse, dq: int, dk: int, dv: int, out_strides, B: int, T: int, n_q: int, n_kv: int,
                 hd: int, window: int, sinks: int, rope) -> None:
     do = _aligned(do)
@@ -149,7 +155,7 @@ def _window_bwd(do, q: int, k: int, v: int, strides, o, lse, dq: int, dk: int, d
     l = native.lib()
     rows = B * n_q * T                                       # scratch: dQ in fp32, sums of the sink rows, delta
     part = rows * hd
-    delta = part + l.tlm_attn_window_part_floats(B, T, n_kv, hd, window, sinks)
+    delta = part + _part_floats(B, T, n_kv, hd, window, sinks)
     work = torch.empty(delta + rows, dtype=torch.float32, device=do.device)
     w = work.data_ptr()
     cos, sin = (t.data_ptr() for t in rope) if rope is not None else (None, None)

@@ -20,6 +20,7 @@ import torch
 
 from . import oracle
 from . import native
+from . import attention_cuda
 
 
 def _use_native(x: torch.Tensor, w: torch.Tensor | None = None) -> bool:
@@ -208,7 +209,7 @@ class _QKVAttention(torch.autograd.Function):
         native.gemm_heads(h, weight, False, dst, 1, B, T, T, Ht, 0, n_q, n_kv, n_q, max(n_kv, 1), hd, n_q + n_kv, cs,
                           tables=(cos, sin))
         if window > 0:
-            o, lse = native.window_attn_fwd_packed(qkv, n_q, n_kv, window, sinks)
+            o, lse = attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks)
         else:
             o, lse = native.flash_attn_fwd(qkv, n_q, n_kv, True)
         ctx.save_for_backward(h, qkv, o, lse, cos, sin)
@@ -221,7 +222,7 @@ class _QKVAttention(torch.autograd.Function):
         n_q, n_kv, window, sinks = ctx.meta
         w = ctx.weight
         if window > 0:
-            d = native.window_attn_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks, rope=(cos, sin))
+            d = attention_cuda.window_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks, rope=(cos, sin))
         else:
             d = native.flash_attn_bwd(do.contiguous(), qkv, o, lse, n_q, n_kv, True, rope=(cos, sin))
         d2 = d.view(h.shape[0], -1)
@@ -333,7 +334,7 @@ def attention_packed(qkv: torch.Tensor, n_q: int, n_kv: int, causal: bool = True
     _check_window(qkv, n_q, n_kv, window, sinks)
     if not (qkv.requires_grad and torch.is_grad_enabled()):
         return _window_packed_fwd(qkv, n_q, n_kv, window, sinks)[0]
-    return _WindowPacked.apply(qkv, n_q, n_kv, window, sinks)
+    return _WindowPacked.apply(qkv, (n_q, n_kv, window, sinks))
 
 
 # --------------------------------------------------------------------------- attention over a sliding window with sinks
@@ -369,10 +370,10 @@ def window_attention_ok(x: torch.Tensor) -> bool:
 
 class _Window(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, window, sinks):
-        ctx.meta = (window, sinks)
+    def forward(ctx, q, k, v, meta):
+        ctx.meta = window, sinks = meta
         if _use_native(q):
-            o, lse = native.window_attn_fwd(q, k, v, window, sinks)
+            o, lse = attention_cuda.window_fwd(q, k, v, window, sinks)
         else:
             o, lse, *_ = _attn_fwd_ref(q, k, v, True, window, sinks)
             o = o.to(q.dtype).contiguous()
@@ -384,24 +385,24 @@ class _Window(torch.autograd.Function):
         q, k, v, o, lse = ctx.saved_tensors
         if _use_native(q):
             out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-            native.window_attn_bwd(do, q, k, v, o, lse, *ctx.meta, out)
+            attention_cuda.window_bwd(do, q, k, v, o, lse, *ctx.meta, out)
         else:
             out = [g.to(q.dtype) for g in _attn_bwd_ref(do, q, k, v, o, True, *ctx.meta)]
-        return *out, None, None
+        return *out, None
 
 
 def _window_packed_fwd(qkv, n_q, n_kv, window, sinks):
     if _use_native(qkv):
-        return native.window_attn_fwd_packed(qkv, n_q, n_kv, window, sinks)
+        return attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks)
     o, lse, *_ = _attn_fwd_ref(*_heads_of(qkv, n_q, n_kv), True, window, sinks)
     return o.to(qkv.dtype).contiguous(), lse
 
 
 class _WindowPacked(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, n_q, n_kv, window, sinks):
-        ctx.meta = (n_q, n_kv, window, sinks)
-        o, lse = _window_packed_fwd(qkv, n_q, n_kv, window, sinks)
+    def forward(ctx, qkv, meta):
+        ctx.meta = meta
+        o, lse = _window_packed_fwd(qkv, *meta)
         ctx.save_for_backward(qkv, o, lse)
         return o
 
@@ -410,10 +411,10 @@ class _WindowPacked(torch.autograd.Function):
         qkv, o, lse = ctx.saved_tensors
         n_q, n_kv, window, sinks = ctx.meta
         if _use_native(qkv):
-            dqkv = native.window_attn_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks)
+            dqkv = attention_cuda.window_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks)
         else:
             dqkv = torch.cat(_attn_bwd_ref(do, *_heads_of(qkv, n_q, n_kv), o, True, window, sinks), dim=2).to(qkv.dtype)
-        return dqkv, None, None, None, None
+        return dqkv, None
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0) -> torch.Tensor:
@@ -427,7 +428,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if q.dtype != k.dtype or q.dtype != v.dtype:
         raise ValueError(f"q, k and v of one type expected, not {q.dtype}, {k.dtype}, {v.dtype}")
     _check_window(q, q.shape[2], k.shape[2], window, sinks, k, v)
-    return _Window.apply(q, k, v, window, sinks)
+    return _Window.apply(q, k, v, (window, sinks))
 
 
 # --------------------------------------------------------------------------- rotary positions, norms of queries and keys
@@ -498,22 +499,22 @@ def _anchors(x, weights):
     """The weights as inputs of a node, only where the node would have no differentiable input without them: their gradients go to
     `main_grad`, and a parameter that is an input ties the node to the stream on which the parameter was first used (a backward
     pass cannot then be captured while an older graph of the same parameters lives)."""
-    return (None, None) if x.requires_grad or weights is None else weights
+    return () if x.requires_grad or weights is None else weights
 
 
 class _QkNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, _q_anchor, _k_anchor, weights, n_q, eps, turn):
+    def forward(ctx, x, args, *anchors):
         ctx.save_for_backward(x)
-        ctx.weights, ctx.n_q, ctx.eps, ctx.turn = weights, n_q, eps, turn
-        turn.keep()
-        return _qk_norm_fwd(x, weights, n_q, eps, turn)
+        ctx.args, ctx.anchors = args, len(anchors)
+        args[3].keep()
+        return _qk_norm_fwd(x, *args)
 
     @staticmethod
     def backward(ctx, dy):
         (x,) = ctx.saved_tensors
-        ctx.turn.check()
-        return _qk_norm_bwd(dy.contiguous(), x, ctx.weights, ctx.n_q, ctx.eps, ctx.turn), None, None, None, None, None, None
+        ctx.args[3].check()
+        return _qk_norm_bwd(dy.contiguous(), x, *ctx.args), None, *(None,) * ctx.anchors
 
 
 def _qk_norm_fwd(x, weights, n_q, eps, turn):
@@ -557,10 +558,11 @@ def qk_norm_rotary(x: torch.Tensor, n_q: int, q_weight: torch.Tensor, k_weight: 
     if not 0 <= n_q <= x.shape[2]:
         raise ValueError(f"n_q {n_q} of {x.shape[2]} heads")
     _check_norm(x, q_weight, k_weight)
-    n_q, eps, turn = int(n_q), float(eps), _Turn(positions, inv_freq, interleaved, scale)
+    weights = (q_weight, k_weight)
+    args = (weights, int(n_q), float(eps), _Turn(positions, inv_freq, interleaved, scale))
     if torch.is_grad_enabled() and (x.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
-        return _QkNormRotary.apply(x, *_anchors(x, (q_weight, k_weight)), (q_weight, k_weight), n_q, eps, turn)
-    return _qk_norm_fwd(x, (q_weight, k_weight), n_q, eps, turn)
+        return _QkNormRotary.apply(x, args, *_anchors(x, weights))
+    return _qk_norm_fwd(x, *args)
 
 
 class _RotaryAttention(torch.autograd.Function):
@@ -569,14 +571,14 @@ class _RotaryAttention(torch.autograd.Function):
     the packed gradient."""
 
     @staticmethod
-    def forward(ctx, qkv, _q_anchor, _k_anchor, weights, n_q, n_kv, eps, turn, window, sinks):
-        ctx.meta = (n_q, n_kv, eps, turn, window, sinks)
-        ctx.weights = weights
+    def forward(ctx, qkv, args, *anchors):
+        ctx.args, ctx.anchors = args, len(anchors)
+        weights, n_q, n_kv, eps, turn, window, sinks = args
         turn.keep()
         raw, v = qkv[:, :, :n_q + n_kv], qkv[:, :, n_q + n_kv:]
-        qk = _turn(raw, turn) if ctx.weights is None else _qk_norm_fwd(raw, ctx.weights, n_q, eps, turn)
+        qk = _turn(raw, turn) if weights is None else _qk_norm_fwd(raw, weights, n_q, eps, turn)
         if _use_native(qkv):
-            o, lse = native.window_attn_fwd(qk[:, :, :n_q], qk[:, :, n_q:], v, window, sinks)
+            o, lse = attention_cuda.window_fwd(qk[:, :, :n_q], qk[:, :, n_q:], v, window, sinks)
         else:
             o, lse, *_ = _attn_fwd_ref(qk[:, :, :n_q], qk[:, :, n_q:], v, True, window, sinks)
             o = o.to(qkv.dtype).contiguous()
@@ -586,23 +588,23 @@ class _RotaryAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do):
         qkv, qk, o, lse = ctx.saved_tensors
-        n_q, n_kv, eps, turn, window, sinks = ctx.meta
+        weights, n_q, n_kv, eps, turn, window, sinks = ctx.args
         turn.check()
         n_qk = n_q + n_kv
         q, k, v = qk[:, :, :n_q], qk[:, :, n_q:], qkv[:, :, n_qk:]
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         if _use_native(qkv):
-            native.window_attn_bwd(do, q, k, v, o, lse, window, sinks, _heads_of(dqkv, n_q, n_kv))
+            attention_cuda.window_bwd(do, q, k, v, o, lse, window, sinks, _heads_of(dqkv, n_q, n_kv))
         else:
             torch.cat(_attn_bwd_ref(do, q, k, v, o, True, window, sinks), dim=2, out=dqkv)
         d = dqkv[:, :, :n_qk]
-        if ctx.weights is not None:
-            _qk_norm_bwd(d, qkv[:, :, :n_qk], ctx.weights, n_q, eps, turn, out=d)
+        if weights is not None:
+            _qk_norm_bwd(d, qkv[:, :, :n_qk], weights, n_q, eps, turn, out=d)
         elif _use_native(qkv):
             native.qk_rotary(d, turn.positions, turn.inv_freq, interleaved=turn.interleaved, scale=turn.scale, inverse=True, out=d)
         else:
             d.copy_(_turn(d, turn, inverse=True))
-        return dqkv, None, None, None, None, None, None, None, None, None
+        return dqkv, None, *(None,) * ctx.anchors
 
 
 def rotary_attention(qkv: torch.Tensor, n_q: int, n_kv: int, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False,
@@ -616,8 +618,8 @@ def rotary_attention(qkv: torch.Tensor, n_q: int, n_kv: int, positions: torch.Te
     if norm_weights is not None:
         norm_weights = tuple(norm_weights)
         _check_norm(qkv, *norm_weights)
-    return _RotaryAttention.apply(qkv, *_anchors(qkv, norm_weights), norm_weights, n_q, n_kv, float(eps),
-                                  _Turn(positions, inv_freq, interleaved, scale), window, sinks)
+    args = (norm_weights, n_q, n_kv, float(eps), _Turn(positions, inv_freq, interleaved, scale), window, sinks)
+    return _RotaryAttention.apply(qkv, args, *_anchors(qkv, norm_weights))
 
 
 # --------------------------------------------------------------------------- SwiGLU

@@ -9,6 +9,7 @@ or unloadable library is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -434,6 +435,11 @@ def rope_qk(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot: int,
 _LL3, _LL9 = _c.c_longlong * 3, _c.c_longlong * 9
 
 
+@functools.lru_cache(maxsize=None)
+def _qk_norm_work_floats(hd: int) -> int:
+    return lib().tlm_qk_norm_work_floats(hd)
+
+
 def qk_rotary(x, positions, inv_freq, weights=None, n_q: int = 0, eps: float = 0.0, interleaved: bool = False, scale: float = 1.0,
               inverse: bool = False, out=None) -> torch.Tensor:
     """`x [B, T, H, hd]` bf16 (rows contiguous) rotated by `positions` (int64, `[T]` or `[B, T]`) and `inv_freq` (float64), with
@@ -456,7 +462,7 @@ def qk_norm_rotary_bwd(dy, x, positions, inv_freq, weights, grads, n_q: int, eps
         out = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=x.device)
     for g in grads:
         assert g.dtype == torch.float32 and g.shape == (hd,) and g.is_contiguous() and g.device == x.device
-    work = torch.empty(lib().tlm_qk_norm_work_floats(hd), dtype=torch.float32, device=x.device)
+    work = torch.empty(_qk_norm_work_floats(hd), dtype=torch.float32, device=x.device)
     _check(lib().tlm_qk_norm_rotary_bwd(x.data_ptr(), _LL3(*x.stride()[:3]), dy.data_ptr(), _LL3(*dy.stride()[:3]), out.data_ptr(),
                                         _LL3(*out.stride()[:3]), positions.data_ptr(), T if positions.dim() > 1 else 0,
                                         inv_freq.data_ptr(), inv_freq.shape[0], weights[0].data_ptr(), weights[1].data_ptr(),
@@ -567,26 +573,6 @@ def flash_attn_bwd(do, qkv, o, lse, n_q: int, n_kv: int, causal: bool, rope=None
     the gradient of the un-rotated q and k (done in fp32 as the gradients leave the kernels)."""
     from . import attention_cuda
     return attention_cuda.bwd(do, qkv, o, lse, n_q, n_kv, causal, rope)
-
-
-def window_attn_fwd(q, k, v, window: int, sinks: int):
-    from . import attention_cuda
-    return attention_cuda.window_fwd(q, k, v, window, sinks)
-
-
-def window_attn_fwd_packed(qkv, n_q: int, n_kv: int, window: int, sinks: int):
-    from . import attention_cuda
-    return attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks)
-
-
-def window_attn_bwd(do, q, k, v, o, lse, window: int, sinks: int, out, rope=None) -> None:
-    from . import attention_cuda
-    attention_cuda.window_bwd(do, q, k, v, o, lse, window, sinks, out, rope)
-
-
-def window_attn_bwd_packed(do, qkv, o, lse, n_q: int, n_kv: int, window: int, sinks: int, rope=None) -> torch.Tensor:
-    from . import attention_cuda
-    return attention_cuda.window_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks, rope)
 
 
 # --------------------------------------------------------------------------- grouped GEMMs (MoE experts)
