@@ -135,12 +135,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _window_fwd(q: int, k: int, v: int, strides, B: int, T: int, n_q: int, n_kv: int, hd: int, window: int, sinks: int, device):
+def _window_fwd(q: int, k: int, v: int, strides, B: int, T: int, n_q: int, n_kv: int, hd: int, window: int, sinks: int, device,
+                rest: bool):
     o = torch.empty((B, T, n_q, hd), dtype=torch.bfloat16, device=device)
+    rest = rest and min(T, (window or T) + sinks) < 128             # no row sees a tile of keys
+    o_rest = torch.empty((B, T, n_q, hd), dtype=torch.bfloat16, device=device) if rest else None
     lse = torch.empty((B, n_q, T), dtype=torch.float32, device=device)
-    native._check(native.lib().tlm_attn_window_fwd(q, k, v, strides, o.data_ptr(), lse.data_ptr(), B, T, n_q, n_kv, hd,
-                                                   1.0 / math.sqrt(hd), min(window, T), min(sinks, T), native._stream()), "attn_window_fwd")
-    return o, lse
+    native._check(native.lib().tlm_attn_window_fwd(q, k, v, strides, o.data_ptr(), native._ptr(o_rest), lse.data_ptr(), B, T, n_q,
+                                                   n_kv, hd, 1.0 / math.sqrt(hd), min(window, T), min(sinks, T), native._stream()), "attn_window_fwd")
+    return o, lse, o_rest
 
 
 @functools.lru_cache(maxsize=1024)
@@ -148,7 +151,7 @@ def _part_floats(B: int, T: int, n_kv: int, hd: int, window: int, sinks: int) ->
     return native.lib().tlm_attn_window_part_floats(B, T, n_kv, hd, window, sinks)
 
 
-def _window_bwd(do, q: int, k: int, v: int, strides, o, lse, dq: int, dk: int, dv: int, out_strides, B: int, T: int, n_q: int, n_kv: int,
+def _window_bwd(do, q: int, k: int, v: int, strides, o, lse, o_rest, dq: int, dk: int, dv: int, out_strides, B: int, T: int, n_q: int, n_kv: int,
                 hd: int, window: int, sinks: int, rope) -> None:
     do = _aligned(do)
     window, sinks = min(window, T), min(sinks, T)
@@ -159,7 +162,7 @@ def _window_bwd(do, q: int, k: int, v: int, strides, o, lse, dq: int, dk: int, d
     work = torch.empty(delta + rows, dtype=torch.float32, device=do.device)
     w = work.data_ptr()
     cos, sin = (t.data_ptr() for t in rope) if rope is not None else (None, None)
-    native._check(l.tlm_attn_window_bwd(q, k, v, strides, o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq, dk, dv, out_strides, w,
+    native._check(l.tlm_attn_window_bwd(q, k, v, strides, o.data_ptr(), native._ptr(o_rest), do.data_ptr(), lse.data_ptr(), dq, dk, dv, out_strides, w,
                                         w + 4 * delta, w + 4 * part, B, T, n_q, n_kv, hd, 1.0 / math.sqrt(hd), cos, sin, window, sinks,
                                         native._stream()), "attn_window_bwd")
 
@@ -172,35 +175,37 @@ def _packed(qkv: torch.Tensor, n_q: int, n_kv: int):
     return p, p + n_q * head, p + (n_q + n_kv) * head, native._LL9(*s, *s, *s)
 
 
-def window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int):
+def window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int, rest: bool = False):
     """Causal attention of `q [B, T, Hq, hd]` over `k`, `v [B, T, Hkv, hd]` (bf16, hd 32 / 64 / 128, strided) where a query sees
-    `window` keys, itself included (0: all), and the first `sinks`. -> o `[B, T, Hq, hd]` bf16, lse `[B, Hq, T]` fp32."""
+    `window` keys, itself included (0: all), and the first `sinks`. -> o `[B, T, Hq, hd]` bf16, lse `[B, Hq, T]` fp32 and, with `rest`,
+    what rounding took off o (bf16, for the backward; None over many keys)."""
     q, k, v = _tiled(q), _tiled(k), _tiled(v)
     B, T, n_q, hd = q.shape
     strides = native._LL9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-    return _window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, B, T, n_q, k.shape[2], hd, window, sinks, q.device)
+    return _window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, B, T, n_q, k.shape[2], hd, window, sinks, q.device,
+                       rest)
 
 
-def window_fwd_packed(qkv: torch.Tensor, n_q: int, n_kv: int, window: int, sinks: int):
+def window_fwd_packed(qkv: torch.Tensor, n_q: int, n_kv: int, window: int, sinks: int, rest: bool = False):
     """The same on the heads of `qkv [B, T, n_q + 2 n_kv, hd]`."""
     qkv = _tiled(qkv)
     B, T, _, hd = qkv.shape
-    return _window_fwd(*_packed(qkv, n_q, n_kv), B, T, n_q, n_kv, hd, window, sinks, qkv.device)
+    return _window_fwd(*_packed(qkv, n_q, n_kv), B, T, n_q, n_kv, hd, window, sinks, qkv.device, rest)
 
 
-def window_bwd(do, q, k, v, o, lse, window: int, sinks: int, out, rope=None) -> None:
+def window_bwd(do, q, k, v, o, lse, o_rest, window: int, sinks: int, out, rope=None) -> None:
     """Gradients of `window_fwd` into `out = (dq, dk, dv)` (bf16, rows contiguous, 16-byte aligned). `rope`: as in `bwd`."""
     q, k, v = _tiled(q), _tiled(k), _tiled(v)
     B, T, n_q, hd = q.shape
     strides, out_strides = (native._LL9(*a.stride()[:3], *b.stride()[:3], *c.stride()[:3]) for a, b, c in ((q, k, v), out))
-    _window_bwd(do, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o, lse, *(t.data_ptr() for t in out), out_strides, B, T, n_q,
+    _window_bwd(do, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o, lse, o_rest, *(t.data_ptr() for t in out), out_strides, B, T, n_q,
                 k.shape[2], hd, window, sinks, rope)
 
 
-def window_bwd_packed(do, qkv, o, lse, n_q: int, n_kv: int, window: int, sinks: int, rope=None) -> torch.Tensor:
+def window_bwd_packed(do, qkv, o, lse, o_rest, n_q: int, n_kv: int, window: int, sinks: int, rope=None) -> torch.Tensor:
     """-> gradient of the packed tensor."""
     qkv = _tiled(qkv)
     B, T, H, hd = qkv.shape
     dqkv = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=qkv.device)
-    _window_bwd(do, *_packed(qkv, n_q, n_kv), o, lse, *_packed(dqkv, n_q, n_kv), B, T, n_q, n_kv, hd, window, sinks, rope)
+    _window_bwd(do, *_packed(qkv, n_q, n_kv), o, lse, o_rest, *_packed(dqkv, n_q, n_kv), B, T, n_q, n_kv, hd, window, sinks, rope)
     return dqkv

@@ -201,34 +201,35 @@ class _QKVAttention(torch.autograd.Function):
     fp32 accumulator, dK as it leaves tensor memory) instead of running a separate pass over the packed gradient."""
 
     @staticmethod
-    def forward(ctx, h, weight, cos, sin, cs, B, T, n_q, n_kv, hd, window, sinks):
+    def forward(ctx, h, weight, cos, sin, cs, B, T, n_q, n_kv, hd, window, sinks, grads):
         Ht = n_q + 2 * n_kv
         qkv = torch.empty(B, T, Ht, hd, dtype=torch.bfloat16, device=h.device)
         import ctypes
         dst = (ctypes.c_void_p * 1)(qkv.data_ptr())
         native.gemm_heads(h, weight, False, dst, 1, B, T, T, Ht, 0, n_q, n_kv, n_q, max(n_kv, 1), hd, n_q + n_kv, cs,
                           tables=(cos, sin))
+        rest = None
         if window > 0:
-            o, lse = attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks)
+            o, lse, rest = attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks, grads)
         else:
             o, lse = native.flash_attn_fwd(qkv, n_q, n_kv, True)
-        ctx.save_for_backward(h, qkv, o, lse, cos, sin)
+        ctx.save_for_backward(h, qkv, o, lse, cos, sin, rest)
         ctx.weight, ctx.meta = weight, (n_q, n_kv, window, sinks)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        h, qkv, o, lse, cos, sin = ctx.saved_tensors
+        h, qkv, o, lse, cos, sin, rest = ctx.saved_tensors
         n_q, n_kv, window, sinks = ctx.meta
         w = ctx.weight
         if window > 0:
-            d = attention_cuda.window_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks, rope=(cos, sin))
+            d = attention_cuda.window_bwd_packed(do, qkv, o, lse, rest, n_q, n_kv, window, sinks, rope=(cos, sin))
         else:
             d = native.flash_attn_bwd(do.contiguous(), qkv, o, lse, n_q, n_kv, True, rope=(cos, sin))
         d2 = d.view(h.shape[0], -1)
         native.gemm_tn_accum(d2, h, _main_grad(w))
         dh = native.gemm_nn(d2, w) if ctx.needs_input_grad[0] else None
-        return dh, None, None, None, None, None, None, None, None, None, None, None
+        return dh, None, None, None, None, None, None, None, None, None, None, None, None
 
 
 def _table(t: torch.Tensor) -> torch.Tensor:
@@ -241,7 +242,7 @@ def _table(t: torch.Tensor) -> torch.Tensor:
 def qkv_attention(h, weight, cos, sin, cs, B: int, T: int, n_q: int, n_kv: int, hd: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
     """CUDA only (same conditions as `qkv_project`): projection + RoPE + causal attention (over a window, see `attention_packed`)
     -> `[B, T, n_q, hd]`."""
-    return _QKVAttention.apply(h, weight, _table(cos), _table(sin), cs, B, T, n_q, n_kv, hd, window, sinks)
+    return _QKVAttention.apply(h, weight, _table(cos), _table(sin), cs, B, T, n_q, n_kv, hd, window, sinks, torch.is_grad_enabled())
 
 
 def qkv_project_fused_ok(h: torch.Tensor, weight: torch.Tensor | None, hd: int, T: int) -> bool:
@@ -373,45 +374,45 @@ class _Window(torch.autograd.Function):
     def forward(ctx, q, k, v, meta):
         ctx.meta = window, sinks = meta
         if _use_native(q):
-            o, lse = attention_cuda.window_fwd(q, k, v, window, sinks)
+            o, lse, rest = attention_cuda.window_fwd(q, k, v, window, sinks, rest=True)
         else:
             o, lse, *_ = _attn_fwd_ref(q, k, v, True, window, sinks)
-            o = o.to(q.dtype).contiguous()
-        ctx.save_for_backward(q, k, v, o, lse)
+            o, rest = o.to(q.dtype).contiguous(), None
+        ctx.save_for_backward(q, k, v, o, lse, rest)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, o, lse, rest = ctx.saved_tensors
         if _use_native(q):
             out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-            attention_cuda.window_bwd(do, q, k, v, o, lse, *ctx.meta, out)
+            attention_cuda.window_bwd(do, q, k, v, o, lse, rest, *ctx.meta, out)
         else:
             out = [g.to(q.dtype) for g in _attn_bwd_ref(do, q, k, v, o, True, *ctx.meta)]
         return *out, None
 
 
-def _window_packed_fwd(qkv, n_q, n_kv, window, sinks):
+def _window_packed_fwd(qkv, n_q, n_kv, window, sinks, rest=False):
     if _use_native(qkv):
-        return attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks)
+        return attention_cuda.window_fwd_packed(qkv, n_q, n_kv, window, sinks, rest)
     o, lse, *_ = _attn_fwd_ref(*_heads_of(qkv, n_q, n_kv), True, window, sinks)
-    return o.to(qkv.dtype).contiguous(), lse
+    return o.to(qkv.dtype).contiguous(), lse, None
 
 
 class _WindowPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, meta):
         ctx.meta = meta
-        o, lse = _window_packed_fwd(qkv, *meta)
-        ctx.save_for_backward(qkv, o, lse)
+        o, lse, rest = _window_packed_fwd(qkv, *meta, rest=True)
+        ctx.save_for_backward(qkv, o, lse, rest)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        qkv, o, lse = ctx.saved_tensors
+        qkv, o, lse, rest = ctx.saved_tensors
         n_q, n_kv, window, sinks = ctx.meta
         if _use_native(qkv):
-            dqkv = attention_cuda.window_bwd_packed(do, qkv, o, lse, n_q, n_kv, window, sinks)
+            dqkv = attention_cuda.window_bwd_packed(do, qkv, o, lse, rest, n_q, n_kv, window, sinks)
         else:
             dqkv = torch.cat(_attn_bwd_ref(do, *_heads_of(qkv, n_q, n_kv), o, True, window, sinks), dim=2).to(qkv.dtype)
         return dqkv, None
@@ -428,6 +429,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if q.dtype != k.dtype or q.dtype != v.dtype:
         raise ValueError(f"q, k and v of one type expected, not {q.dtype}, {k.dtype}, {v.dtype}")
     _check_window(q, q.shape[2], k.shape[2], window, sinks, k, v)
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        if _use_native(q):
+            return attention_cuda.window_fwd(q, k, v, window, sinks)[0]
+        return _attn_fwd_ref(q, k, v, True, window, sinks)[0].to(q.dtype).contiguous()
     return _Window.apply(q, k, v, (window, sinks))
 
 
@@ -573,28 +578,28 @@ class _RotaryAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, args, *anchors):
         ctx.args, ctx.anchors = args, len(anchors)
-        weights, n_q, n_kv, eps, turn, window, sinks = args
+        weights, n_q, n_kv, eps, turn, window, sinks, grads = args
         turn.keep()
         raw, v = qkv[:, :, :n_q + n_kv], qkv[:, :, n_q + n_kv:]
         qk = _turn(raw, turn) if weights is None else _qk_norm_fwd(raw, weights, n_q, eps, turn)
         if _use_native(qkv):
-            o, lse = attention_cuda.window_fwd(qk[:, :, :n_q], qk[:, :, n_q:], v, window, sinks)
+            o, lse, rest = attention_cuda.window_fwd(qk[:, :, :n_q], qk[:, :, n_q:], v, window, sinks, grads)
         else:
             o, lse, *_ = _attn_fwd_ref(qk[:, :, :n_q], qk[:, :, n_q:], v, True, window, sinks)
-            o = o.to(qkv.dtype).contiguous()
-        ctx.save_for_backward(qkv, qk, o, lse)
+            o, rest = o.to(qkv.dtype).contiguous(), None
+        ctx.save_for_backward(qkv, qk, o, lse, rest)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        qkv, qk, o, lse = ctx.saved_tensors
-        weights, n_q, n_kv, eps, turn, window, sinks = ctx.args
+        qkv, qk, o, lse, rest = ctx.saved_tensors
+        weights, n_q, n_kv, eps, turn, window, sinks, _ = ctx.args
         turn.check()
         n_qk = n_q + n_kv
         q, k, v = qk[:, :, :n_q], qk[:, :, n_q:], qkv[:, :, n_qk:]
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         if _use_native(qkv):
-            attention_cuda.window_bwd(do, q, k, v, o, lse, window, sinks, _heads_of(dqkv, n_q, n_kv))
+            attention_cuda.window_bwd(do, q, k, v, o, lse, rest, window, sinks, _heads_of(dqkv, n_q, n_kv))
         else:
             torch.cat(_attn_bwd_ref(do, q, k, v, o, True, window, sinks), dim=2, out=dqkv)
         d = dqkv[:, :, :n_qk]
@@ -618,7 +623,7 @@ def rotary_attention(qkv: torch.Tensor, n_q: int, n_kv: int, positions: torch.Te
     if norm_weights is not None:
         norm_weights = tuple(norm_weights)
         _check_norm(qkv, *norm_weights)
-    args = (norm_weights, n_q, n_kv, float(eps), _Turn(positions, inv_freq, interleaved, scale), window, sinks)
+    args = (norm_weights, n_q, n_kv, float(eps), _Turn(positions, inv_freq, interleaved, scale), window, sinks, torch.is_grad_enabled())
     return _RotaryAttention.apply(qkv, args, *_anchors(qkv, norm_weights))
 
 
