@@ -21,6 +21,20 @@ def plan(tmp_path_factory):
     return exe
 
 
+def test_pieces_of_many_sink_tiles_stay_few(tmp_path):
+    """A piece of a sink tile leaves 128 rows of partial sums: 256 pieces in all while there are fewer tiles, else one a tile."""
+    if shutil.which("g++") is None:
+        pytest.skip("no host compiler")
+    src, exe = tmp_path / "far.cpp", str(tmp_path / "far")
+    src.write_text('#include <cstdio>\n#include "window_plan.h"\nint main() { int T, W, S; while (std::scanf("%d %d %d", &T, &W, &S) == 3) '
+                   '{ const tlm::WinFar f = tlm::win_far(T, W, S); std::printf("%d %d\\n", f.tiles, f.chunks); } }\n')
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", SRC, str(src), "-o", exe], check=True)
+    cases = [(T, W, S) for T in (4096, 32768, 131072, 1 << 20, 1 << 29) for W in (1, 1024) for S in (1, 129, 1000, T // 8, T // 2, T)]
+    out = subprocess.run([exe], input="".join("%d %d %d\n" % c for c in cases), capture_output=True, text=True, check=True).stdout.split()
+    for (T, W, S), tiles, chunks in zip(cases, map(int, out[::2]), map(int, out[1::2])):
+        assert chunks >= 1 and 1 <= tiles <= -(-S // 128) and tiles * chunks <= max(256, tiles) and chunks <= 64, (T, W, S, tiles, chunks)
+
+
 def test_every_visible_pair_is_met_once(plan):
     rng = random.Random(0)
     sizes = [1, 2, 127, 128, 129, 255, 256, 257, 640, 1001]

@@ -39,19 +39,20 @@ struct WinFar {
   int tiles;           // sink tiles that have far query tiles
   int chunk, chunks;   // query tiles a piece, pieces of tile 0 (which has the most)
 };
-// A piece is as long as a block's share of the window, but not below 8 query tiles (a block costs about 5 steps beside its steps) and
-// at most 64 pieces (they are added up one by one).
+// A piece is as long as a block's share of the window, but not below 8 query tiles (a block costs about 5 steps beside its steps).
+// There are at most 64 of a tile, which are added up one by one, and 256 in all, or one a tile: each holds its tile's rows in memory. In
+// us, 64 of every tile / 256 / 64 in all (16 / 8 heads of 64): 32768 keys and 16384 sinks, window 1024 6908 / 5426 / 5345 and 1.9 GB /
+// 201 / 134 MB, 1000 sinks 1020 / 978 / 936; 8192 keys, 2000 sinks, window 256, 4 / 1 heads 87 / 89 / 102.
 TLM_TILE_HD WinFar win_far(int T, int W, int S) {
   const int n_tiles = (T + WIN_TILE - 1) / WIN_TILE, far0 = S > 0 ? n_tiles - 1 - win_last_q(0, W, n_tiles) : 0;
   WinFar f{0, 1, 0};
   if (far0 <= 0) return f;
-  int chunk = 1 + (WIN_TILE - 2 + W) / WIN_TILE;
-  if (chunk < 8) chunk = 8;
-  if (chunk < (far0 + 63) / 64) chunk = (far0 + 63) / 64;
-  f.chunk = chunk;
-  f.chunks = (far0 + chunk - 1) / chunk;
   f.tiles = (S + WIN_TILE - 1) / WIN_TILE;
-  while (f.tiles > 0 && win_last_q(f.tiles - 1, W, n_tiles) >= n_tiles - 1) --f.tiles;
+  while (win_last_q(f.tiles - 1, W, n_tiles) >= n_tiles - 1) --f.tiles;       // tile 0 has far0 > 0
+  const int most = f.tiles < 4 ? 64 : f.tiles < 256 ? 256 / f.tiles : 1, share = 1 + (WIN_TILE - 2 + W) / WIN_TILE;
+  f.chunk = share < 8 ? 8 : share;
+  if (f.chunk < (far0 + most - 1) / most) f.chunk = (far0 + most - 1) / most;
+  f.chunks = (far0 + f.chunk - 1) / f.chunk;
   return f;
 }
 // Query tiles [from, to) of piece c of sink tile j (none where from >= to)
