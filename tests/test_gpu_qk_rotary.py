@@ -168,3 +168,29 @@ def test_refusals():
     with pytest.raises(ValueError, match="weights"):
         F_ops.qk_norm_rotary(x, 2, w[0].float(), w[1], pos, freq)
     assert F_ops.rotary(x[:, :0], pos[:0], freq).shape == (2, 0, 4, 64)
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of a tensor of more than 2^31 elements, as they come out alone."""
+    from train_large_model_from_scratch_b200.ops import functional as F_ops, native
+    T, heads, d, n = 140032, 120, 128, 40
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(1, T, heads, d, generator=gen, device="cuda").bfloat16()
+    pos, freq = torch.arange(T, device="cuda"), 10000.0 ** (-torch.arange(d // 2, device="cuda", dtype=torch.float64) * 2 / d)
+    w = [(1 + 0.5 * torch.randn(d, generator=gen, device="cuda")).bfloat16() for _ in range(2)]
+    for leaf_w in w:
+        leaf_w.main_grad = torch.zeros(d, device="cuda")
+
+    def run(x, pos):
+        x = x.detach().requires_grad_()
+        y = F_ops.qk_norm_rotary(x, 96, *w, pos, freq)
+        (dx,) = torch.autograd.grad(y, x, x.detach())
+        return y.detach()[:, -n:].clone(), dx[:, -n:].clone(), F_ops.rotary(x.detach(), pos, freq)[:, -n:].clone()
+
+    got, want = run(x, pos), run(x[:, -n:].contiguous(), pos[-n:])
+    native.raise_on_device_status()
+    assert x.numel() > 2 ** 31
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

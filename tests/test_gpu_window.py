@@ -295,3 +295,21 @@ def test_refusals():
         F_ops.window_attention(q, k.cpu(), v, window=4)
     empty = F_ops.window_attention(q[:, :0], k[:, :0], v[:, :0], window=4)
     assert empty.shape == (1, 0, 2, 64)
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of a tensor of more than 2^31 elements: as those of its end alone, which no earlier key reaches. Probabilities, dS
+    and each output row's terms are the same; sums in another order may round to the other side: one bf16 step."""
+    T, n, n_q, n_kv, d, window = 140032, 512, 104, 8, 128, 100
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    qkv, do = _inputs(1, T, n_q, n_kv, d)
+    want = _run_packed(qkv[:, -n:].contiguous(), do[:, -n:].contiguous(), n_q, n_kv, window, 0)
+    from train_large_model_from_scratch_b200.ops import functional as F_ops, native
+    o = F_ops.attention_packed(qkv.requires_grad_(), n_q, n_kv, window=window)
+    (g,) = torch.autograd.grad(o, qkv, do)
+    native.raise_on_device_status()
+    assert qkv.numel() > 2 ** 31 and g.shape == qkv.shape
+    for name, a, b in zip(("o", "dq", "dk", "dv"), (o.detach(), *g.split([n_q, n_kv, n_kv], dim=2)), want):
+        a, b = a[:, 128 - n:].double(), b[:, 128:].double()
+        assert ((a - b).abs() <= 2 * H * b.abs() + 2.0 ** -18 * b.abs().max()).all(), name
