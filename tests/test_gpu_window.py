@@ -21,6 +21,10 @@ def _reference(q, k, v, do, window, sinks):
     p = torch.softmax((q @ k.mT / math.sqrt(d)).masked_fill(~seen, -math.inf), dim=-1)
     o = p @ v
     eo = H * (p @ v.abs() + o.abs())
+    if min(T, (window or T) + sinks) < 128:
+        # divided by the sum of the rounded probabilities: sum p (1 + e_j) v_j / sum p (1 + e_j) = o + sum p e_j (v_j - o) + O(e^2), |e_j| <= H,
+        # and |v_j - o| <= |v_j| + |o|
+        eo = eo + H * o.abs()
     dp = do @ v.mT
     ds = p * (dp - (p * dp).sum(-1, keepdim=True))
     eds = H * ds.abs() + p * (do.abs() * eo).sum(-1, keepdim=True)

@@ -492,9 +492,10 @@ class _Rotary(torch.autograd.Function):
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
-    """Every head of `x [B, T, H, hd]` turned by its token's position: `positions` int64 `[T]` or `[B, T]` (any values), `inv_freq`
-    and `scale` from `oracle.rotary_frequencies`. The first `2 * len(inv_freq)` elements of a head turn, in pairs
-    (i, i + len(inv_freq)) or, `interleaved`, (2 i, 2 i + 1); the rest passes. A new tensor; `x` may be a view (rows contiguous)."""
+    """Every head of `x [B, T, H, hd]` turned by its token's position: `positions` int64 `[T]` or `[B, T]` (any values; an angle is off by
+    a few 2^-53 of itself), `inv_freq` and `scale` from `oracle.rotary_frequencies`. The first `2 * len(inv_freq)` elements of a head
+    turn, in pairs (i, i + len(inv_freq)) or, `interleaved`, (2 i, 2 i + 1); the rest passes. A new tensor; `x` may be a view (rows
+    contiguous)."""
     x, positions, inv_freq = _check_rotary(x, positions, inv_freq)
     turn = _Turn(positions, inv_freq, interleaved, scale)
     return _Rotary.apply(x, turn) if x.requires_grad and torch.is_grad_enabled() else _turn(x, turn)
