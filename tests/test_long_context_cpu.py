@@ -133,6 +133,20 @@ def test_frequencies():
             oracle.rotary_frequencies(**bad)
 
 
+@pytest.mark.parametrize("dim,theta,length,factor,low,high", [
+    # low, high: the pairs floor(dim ln(length / 64 pi) / 2 ln(theta)) and ceil(dim ln(length / 2 pi) / 2 ln(theta)), worked out by hand
+    (8, 10000.0, 8192, 8.0, 1, 4),           # 1.61 and 3.12: the last pair (3) turns 1.30 times and is on the ramp
+    (64, 10000.0, 131072, 8.0, 22, 35),      # 22.51 and 34.55
+    (16, 10000.0, 32768, 4.0, 4, 8),         # 4.42 and 7.43
+    (64, 10000.0, 4096, 8.0, 10, 23),        # 10.47 and 22.51: ends inside the head
+    (4, 10.0, 1 << 20, 2.0, 7, 3)])          # 7.43 and 10.45, at most dim - 1: every pair turns more than 32 times and stays
+def test_the_ramp_may_end_behind_the_last_pair(dim, theta, length, factor, low, high):
+    freq = oracle.rotary_frequencies(dim, theta, "yarn", factor, length)[0].tolist()
+    for i, f in enumerate(freq):
+        part = min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0)          # of the way from 1 to 1 / factor
+        assert abs(f * theta ** (2 * i / dim) - (1 - part + part / factor)) < 1e-12, i
+
+
 def test_refusals():
     qkv, pos, freq, w = _randn(1, 4, 4, 8), torch.arange(4), torch.ones(4, dtype=torch.float64), torch.ones(8)
     for call, match in (

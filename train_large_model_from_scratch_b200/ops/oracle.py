@@ -74,7 +74,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "
 
     scaling "linear": positions are divided by `factor`. "ntk": theta grows so that the slowest pair turns `factor` times slower.
     "yarn": pairs that turn more than 32 times within `original_length` stay, those below one turn are divided by `factor`, with
-    a linear ramp over the pair index between; cos and sin are multiplied by 0.1 ln(factor) + 1.
+    a linear ramp over the pair index between, which may end behind the last pair (where that turns more than once); cos and sin
+    are multiplied by 0.1 ln(factor) + 1.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, not {rotary_dim}")
@@ -96,7 +97,7 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "
     def pair_of(turns: float) -> float:           # index of the pair that turns so often within original_length
         return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-    low, high = max(0, math.floor(pair_of(32.0))), min(rotary_dim // 2 - 1, math.ceil(pair_of(1.0)))
+    low, high = max(0, math.floor(pair_of(32.0))), min(rotary_dim - 1, math.ceil(pair_of(1.0)))
     ramp = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
     return freq * (1.0 - ramp) + freq / factor * ramp, 0.1 * math.log(factor) + 1.0
 
