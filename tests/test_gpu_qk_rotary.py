@@ -82,6 +82,30 @@ def test_norm_and_rotary(B, T, heads, d, r, per_batch, interleaved):
         assert ((p.main_grad.double() - 3.0 - terms.sum((0, 1, 2))).abs() <= 2.0 ** -17 * (3.0 + terms.abs().sum((0, 1, 2)))).all()
 
 
+@pytest.mark.parametrize("B,T,heads,d", [(1, 1, 1, 64), (1, 7, 12, 64), (2, 5, 3, 32), (1, 33, 5, 128), (3, 3, 7, 96), (1, 3, 2, 22), (1, 700, 5, 256)])
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+def test_an_eps_of_zero(B, T, heads, d, eps):
+    """... or one that is zero in 32 bits: places of a block that have no row add nothing to the weights' gradients."""
+    from train_large_model_from_scratch_b200.ops import functional as F_ops
+    x, dy, pos, freq, w = _case(B, T, heads, d, d, False, seed=6)
+    n_q = heads - heads // 3
+    leaf, params = x.detach().requires_grad_(), [torch.nn.Parameter(t) for t in w]
+    y = F_ops.qk_norm_rotary(leaf, n_q, *params, pos, freq, eps=eps)
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    is_q = (torch.arange(heads, device="cuda") < n_q)[:, None]
+    wt = torch.where(is_q, w[0].double(), w[1].double())
+    rstd = x.double().pow(2).mean(-1, keepdim=True).rsqrt()
+    hat = x.double() * rstd
+    _close(y.detach(), _turn(hat * wt, pos, freq, False, 1.0), 4 * _rowmax(hat * wt))
+    du = _turn(dy, pos, freq, False, 1.0, inverse=True)
+    g = du * wt
+    _close(dx, rstd * (g - hat * (g * hat).mean(-1, keepdim=True)), rstd * 4 * (_rowmax(g) + _rowmax(hat) * (g * hat).abs().mean(-1, keepdim=True)))
+    for p, heads_of in zip(params, (slice(0, n_q), slice(n_q, None))):
+        # du is a difference of two products of dy, each off by a few 2^-24 of its own size
+        terms, size = (du * hat)[:, :, heads_of], (2 * _rowmax(dy.double()) * hat.abs())[:, :, heads_of]
+        assert ((p.main_grad.double() - terms.sum((0, 1, 2))).abs() <= 2.0 ** -17 * terms.abs().sum((0, 1, 2)) + 2.0 ** -20 * size.sum((0, 1, 2))).all()
+
+
 def test_far_positions_keep_their_angle():
     """Around 2^32 a 32-bit angle would say nothing."""
     from train_large_model_from_scratch_b200.ops import functional as F_ops

@@ -171,6 +171,15 @@ def test_refusals():
             call()
 
 
+@pytest.mark.parametrize("eps", [-1e-6, float("nan")])
+def test_a_negative_eps_is_refused(eps):
+    qkv, pos, freq, w = _randn(1, 4, 4, 8), torch.arange(4), torch.ones(4, dtype=torch.float64), torch.ones(8)
+    with pytest.raises(ValueError, match="eps"):
+        Fo.qk_norm_rotary(qkv, 2, w, w, pos, freq, eps=eps)
+    with pytest.raises(ValueError, match="eps"):
+        Fo.rotary_attention(qkv, 2, 1, pos, freq, norm_weights=(w, w), eps=eps)
+
+
 def test_config():
     flags = ["--rope_variant", "standard", "--qk_norm", "--rope_layout", "interleaved", "--rope_fraction", "0.5", "--rope_scaling", "yarn",
              "--rope_scaling_factor", "4", "--attn_window", "64", "--attn_sinks", "4"]

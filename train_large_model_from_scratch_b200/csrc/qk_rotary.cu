@@ -323,9 +323,11 @@ qk_norm_rotary_bwd_kernel(const QrParams p) {
       const bool ok = more ? now.in && h + me.hps < p.H : next.in && me.h0 < p.H;
       rx = map.load(more ? x : x_next, ok);
       rg = map.load(more ? dy : dy_next, ok);
-      const float rstd = rsqrtf(row_sum<LPR>(dot16(v, v)) * inv_hd + p.eps);
+      const bool there = now.in && h < p.H;
+      // a row that is not there adds zeros to the weights' sums: its own rstd is infinite where eps is 0
+      const float mean = row_sum<LPR>(dot16(v, v)) * inv_hd + p.eps, rstd = there ? rsqrtf(mean) : 0.f;
       turn.rotate(g, me);
-      // du * xhat, for the weights; rows that are not there add zeros
+      // du * xhat, for the weights
       if (h < p.n_q) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) { dq.a[j] = ffma2(fmul2(g.a[j], both(rstd)), v.a[j], dq.a[j]); dq.b[j] = ffma2(fmul2(g.b[j], both(rstd)), v.b[j], dq.b[j]); }
@@ -343,7 +345,7 @@ qk_norm_rotary_bwd_kernel(const QrParams p) {
         out.b[j] = ffma2(fmul2(v.b[j], both(rstd)), both(back), g.b[j]);
       }
       scale_by(out, rstd);
-      if (now.in && h < p.H) map.store(dx, pack<INTER>(out));
+      if (there) map.store(dx, pack<INTER>(out));
       dx += p.out.sh * me.hps;
     }
     now = next;

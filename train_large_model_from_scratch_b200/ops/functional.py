@@ -549,7 +549,9 @@ def _qk_norm_bwd(dy, x, weights, n_q, eps, turn, out=None):
     return dx if out is None else out.copy_(dx)
 
 
-def _check_norm(x, *weights) -> None:
+def _check_norm(x, eps, *weights) -> None:
+    if not eps >= 0.0:
+        raise ValueError(f"eps {eps}: it may not be negative")
     for w in weights:
         if tuple(w.shape) != (x.shape[3],) or w.dtype != x.dtype or not w.is_contiguous():
             raise ValueError(f"weights have to be contiguous {x.dtype} [{x.shape[3]}], not {w.dtype} {tuple(w.shape)}")
@@ -563,7 +565,7 @@ def qk_norm_rotary(x: torch.Tensor, n_q: int, q_weight: torch.Tensor, k_weight: 
     x, positions, inv_freq = _check_rotary(x, positions, inv_freq)
     if not 0 <= n_q <= x.shape[2]:
         raise ValueError(f"n_q {n_q} of {x.shape[2]} heads")
-    _check_norm(x, q_weight, k_weight)
+    _check_norm(x, eps, q_weight, k_weight)
     weights = (q_weight, k_weight)
     args = (weights, int(n_q), float(eps), _Turn(positions, inv_freq, interleaved, scale))
     if torch.is_grad_enabled() and (x.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
@@ -623,7 +625,7 @@ def rotary_attention(qkv: torch.Tensor, n_q: int, n_kv: int, positions: torch.Te
     _check_window(qkv, n_q, n_kv, window, sinks)
     if norm_weights is not None:
         norm_weights = tuple(norm_weights)
-        _check_norm(qkv, *norm_weights)
+        _check_norm(qkv, eps, *norm_weights)
     args = (norm_weights, n_q, n_kv, float(eps), _Turn(positions, inv_freq, interleaved, scale), window, sinks, torch.is_grad_enabled())
     return _RotaryAttention.apply(qkv, args, *_anchors(qkv, norm_weights))
 
