@@ -170,6 +170,31 @@ def test_hidden_keys_may_hold_anything_finite():
         assert torch.equal(got[0][:, rows], base[0][:, rows])
 
 
+@pytest.mark.parametrize("split", ["1", "2"])
+@pytest.mark.parametrize("at,window,sinks", [(300, 40, 2), (1, 40, 1), (599, 40, 0), (300, 1000, 0), (130, 140, 130)])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_gradients_beside_a_hidden_value_of_any_size(d, at, window, sinks, split, monkeypatch):
+    """do * v of a hidden key may overflow: neither the gradients of the queries that do not see it, nor those of the keys that none
+    of its queries sees, know of it. dq is reduced in hardware order: one rounding to either side."""
+    from train_large_model_from_scratch_b200.ops import oracle
+    monkeypatch.setenv("TLM_ATTN_BWD_SPLIT", split)
+    n_q, n_kv, T = 2, 1, 600
+    qkv, do = _inputs(1, T, n_q, n_kv, d, seed=11)
+    base = _run_packed(qkv, do, n_q, n_kv, window, sinks)
+    bad = qkv.clone()
+    bad[:, at, n_q + 1] = 3e38
+    got = _run_packed(bad, do, n_q, n_kv, window, sinks)
+    seen = oracle.window_mask(T, window, sinks, "cuda")
+    rows = ~seen[:, at]
+    keys = ~seen[~rows].any(0)
+    assert torch.equal(got[0][:, rows], base[0][:, rows])
+    if rows.any():
+        a, b = got[1][:, rows].float(), base[1][:, rows].float()
+        assert ((a - b).abs() <= 2 * H * b.abs() + 1e-5 * base[1].abs().max()).all()
+    for a, b in zip(got[2:], base[2:]):
+        assert torch.equal(a[:, keys], b[:, keys])
+
+
 @pytest.mark.parametrize("d", [32, 64, 128])
 def test_a_key_of_nan_reaches_the_rows_that_see_it(d):
     """... and no others: a hidden score is hidden whatever it is."""

@@ -35,6 +35,42 @@ def test_pieces_of_many_sink_tiles_stay_few(tmp_path):
         assert chunks >= 1 and 1 <= tiles <= -(-S // 128) and tiles * chunks <= max(256, tiles) and chunks <= 64, (T, W, S, tiles, chunks)
 
 
+def test_blocks_without_a_mask_have_nothing_to_hide(tmp_path):
+    """The backward's 32 x 32 blocks: where one is taken without a mask all its pairs are visible; where not, the columns that a row
+    sees are those of the definition."""
+    if shutil.which("g++") is None:
+        pytest.skip("no host compiler")
+    src, exe = tmp_path / "block.cpp", str(tmp_path / "block")
+    src.write_text("""#include <cstdio>
+#include "window_plan.h"
+int main() {
+  int T, W, S;
+  while (std::scanf("%d %d %d", &T, &W, &S) == 3) {
+    const int n = (T + 127) / 128;
+    int bad = 0;
+    for (int j = 0; j < n; ++j)
+      for (int qi = j; qi < n; ++qi)
+        for (int block = 0; block < 16; ++block) {
+          const int k0 = j * 128 + block / 4 * 32, q0 = qi * 128 + block % 4 * 32;
+          const bool partial = tlm::win_block_partial(j, k0 - q0, W, S);
+          for (int k = k0; k < k0 + 32; ++k)
+            for (int i = 0; i < 32; ++i) {
+              const bool seen = k <= q0 + i && (q0 + i - k < W || k < S);
+              const bool kept = (unsigned)(i - (k - q0)) < (k < S ? 0x80000000u : (unsigned)W);
+              bad += partial ? kept != seen : !seen;
+            }
+        }
+    std::printf("%d\\n", bad);
+  }
+}
+""")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", SRC, str(src), "-o", exe], check=True)
+    cases = [(T, W, S) for T in (1, 100, 128, 400, 700) for W in (1, 2, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129, 160, 300, 700) if W <= T
+             for S in (0, 1, 4, 31, 32, 127, 128, 129, 300) if S <= T]
+    out = subprocess.run([exe], input="".join("%d %d %d\n" % c for c in cases), capture_output=True, text=True, check=True).stdout.split()
+    assert len(out) == len(cases) and not [c for c, o in zip(cases, out) if o != "0"]
+
+
 def test_every_visible_pair_is_met_once(plan):
     rng = random.Random(0)
     sizes = [1, 2, 127, 128, 129, 255, 256, 257, 640, 1001]

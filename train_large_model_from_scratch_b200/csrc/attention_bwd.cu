@@ -27,7 +27,7 @@
 // walks over the query tiles of its KV tile's window; the query tiles that see a tile only as sinks are further blocks, whose
 // dV | dK rows meet the tile's own in an fp32 buffer that the conversion pass adds up in fixed order. A step costs what it does in
 // the causal form; what a short window adds is a block's start and end, about 4 steps of 16 + 4 at B 8, T 4096, 16 / 8 heads of 64,
-// window 1024: 486 us with delta and conversion passes (32 / 4 of 32, window 512 498; B 2, 16 / 4 of 128, window 2048 360).
+// window 1024: 491 us with delta and conversion passes (32 / 4 of 32, window 512 505; B 2, 16 / 4 of 128, window 2048 364).
 // Every wait is bounded; on a timeout the CTA records a status code, leaves its
 // loops and still releases its tensor memory.
 #include "attention_window.h"
@@ -411,6 +411,21 @@ __device__ __forceinline__ void attn_bwd_p(uint32_t t_s, const float* nlse, floa
   }
 }
 
+// Does some thread of the warp have a NaN among its 32 packed dS? A hidden pair's P is zero, but zero times dP - delta is NaN where do * v of
+// the pair or do * o of the row overflow; hidden pairs are cleared then. Looked for behind the stores of dS, while they are on their way,
+// and by warps that have hidden pairs only. In us with delta and conversion passes, without it / so / in front of the stores, in all
+// warps of such tiles / as a select for each of their columns: 8 x 4096, 32 / 4 heads of 32, window 512 499 / 505 / 515 / 524; 16 / 8 of 64,
+// window 1024 489 / 491 / 499 / 501; 2 x 4096, 16 / 4 of 128, window 2048 362 / 364 / 373 / 375.
+__device__ __forceinline__ bool attn_bwd_any_nan(const uint32_t* dd) {
+  const __nv_bfloat162* d = reinterpret_cast<const __nv_bfloat162*>(dd);
+  const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+  __nv_bfloat162 a = d[0], b = d[1];
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) { a = __hfma2(d[i], zero, a); b = __hfma2(d[i + 1], zero, b); }      // a, or NaN
+  const float2 s = __bfloat1622float2(__hfma2(a, zero, b));
+  return __any_sync(0xffffffffu, s.x != s.x || s.y != s.y);
+}
+
 // SPLIT: a cluster of p.split CTAs works on one KV tile, each on its share of the (query head, query tile) steps; every CTA
 // leaves its fp32 dV | dK in its own shared memory and the cluster adds them up, in fixed order. See split_for.
 template <int HD, bool SCATTER, bool SPLIT, bool WIN>
@@ -713,9 +728,12 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
       tc_fence_after();
       float2 pr[16];
       // two copies: the compare and select of the diagonal tiles doubled the instructions of a pair in all the others
+      // WIN: columns [first, first + width) of a row are seen; `masked`: not all of them in all of this warp's rows
+      const int first0 = (j - qi) * AB_TILE + q4 * 32 - s * 64 - col0, first = first0 + lane;
+      const bool masked = WIN && win_block_partial(j, first0, p.window, p.sinks);
+      const uint32_t width = t_row < p.sinks ? 0x80000000u : (uint32_t)p.window;
       if constexpr (WIN) {
-        if (qi == j || ((qi - j) * AB_TILE + AB_TILE - 1 >= p.window && (j + 1) * AB_TILE > p.sinks))
-          attn_bwd_p<true, true>(t_s, rows, sc2, (j - qi) * AB_TILE + row - s * 64 - col0, pr, t_row < p.sinks ? 0x80000000u : (uint32_t)p.window);
+        if (masked) attn_bwd_p<true, true>(t_s, rows, sc2, first, pr, width);
         else attn_bwd_p<false>(t_s, rows, sc2, 0, pr);
       } else if (qi == j) attn_bwd_p<true>(t_s, rows, sc2, row - s * 64 - col0, pr);
       else attn_bwd_p<false>(t_s, rows, sc2, 0, pr);
@@ -745,9 +763,22 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
       }
       tmem_st16(t_s + 16, dd);
       if (!C::WIDE && it > 1 && !mbar_wait_warp(bar(DQ_FULL + (it & 1)), ((uint32_t)(it >> 1) & 1u) ^ 1u, 30, abort_flag, p.status)) { ok = false; break; }
+      auto store_ds = [&] {
 #pragma unroll
-      for (int ch = 0; ch < 4; ++ch)
-        *reinterpret_cast<uint4*>(drow + ((((col0 >> 3) + ch) ^ (row & 7)) << 4)) = make_uint4(dd[4 * ch], dd[4 * ch + 1], dd[4 * ch + 2], dd[4 * ch + 3]);
+        for (int ch = 0; ch < 4; ++ch)
+          *reinterpret_cast<uint4*>(drow + ((((col0 >> 3) + ch) ^ (row & 7)) << 4)) = make_uint4(dd[4 * ch], dd[4 * ch + 1], dd[4 * ch + 2], dd[4 * ch + 3]);
+      };
+      store_ds();
+      if (masked && attn_bwd_any_nan(dd)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if ((uint32_t)(2 * i - first) >= width) dd[i] &= 0xffff0000u;
+          if ((uint32_t)(2 * i + 1 - first) >= width) dd[i] &= 0x0000ffffu;
+        }
+        __syncwarp();
+        tmem_st16(t_s + 16, dd);
+        store_ds();
+      }
       fence_proxy_async_smem();
       tmem_st_wait();
       tc_fence_before();

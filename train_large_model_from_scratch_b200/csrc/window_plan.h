@@ -35,6 +35,12 @@ TLM_TILE_HD int win_last_q(int j, int W, int n_tiles) {
   return last < n_tiles - 1 ? last : n_tiles - 1;
 }
 
+// A warp of the backward takes 32 keys of KV tile j by 32 queries; `ahead` is how far its first key lies behind its first query's own place
+// (negative: in front of it). Query i of key k's row is seen iff ahead + k <= i < ahead + k + W (or whatever, for sinks). Is one hidden?
+TLM_TILE_HD bool win_block_partial(int j, int ahead, int W, int S) {
+  return ahead > -31 || (ahead + W < 32 && (j + 1) * WIN_TILE > S);
+}
+
 struct WinFar {
   int tiles;           // sink tiles that have far query tiles
   int chunk, chunks;   // query tiles a piece, pieces of tile 0 (which has the most)

@@ -422,8 +422,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     """Causal GQA attention of `q [B, T, Hq, hd]` over `k`, `v [B, T, Hkv, hd]` -> `[B, T, Hq, hd]`: key j is visible to query i iff
     j <= i and (i - j < window or j < sinks); `window` 0: no window. The three may be views of one another's storage or of a
     packed tensor; rows that are no whole 16-byte pieces apart are copied first. bf16 on the GPU with head dims 32, 64, 128.
-    Inputs have to be finite where a row's 128 neighbours look: a hidden key's weight is exactly zero, but zero times an infinite
-    or NaN value is NaN."""
+    Hidden keys and values may hold anything finite, for the output and the gradients of what does not see them. Inputs have to be
+    finite where a row's 128 neighbours look: a hidden key's weight is exactly zero, but zero times an infinite or NaN value is
+    NaN."""
     if q.dim() != 4 or k.shape != v.shape or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q [B, T, Hq, hd] with k and v [B, T, Hkv, hd] expected, not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype != k.dtype or q.dtype != v.dtype:
