@@ -229,6 +229,30 @@ def test_rows_with_few_keys_keep_their_gradients(T, window, sinks, d):
     assert worst <= 3 * H, worst
 
 
+@pytest.mark.parametrize("T,window,sinks", [(128, 1000, 0), (129, 128, 0), (300, 1000, 0), (300, 200, 4), (260, 100, 60), (700, 1, 127)])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_the_first_rows_of_a_long_window_keep_their_gradients(T, window, sinks, d):
+    """A sequence's first rows see few keys whatever the window. Row by row, dS = p (dp - delta): delta is a weighted mean of dp whose
+    weights are off by half a bf16 step each, so off by at most that of sum p |dp - delta|; dS and dq are rounded once; o in delta is
+    held to 2^-17, sums of products to 2^-18 of their terms."""
+    qkv, do = _inputs(2, T, 16, 8, d, seed=40)
+    got = _run_packed(qkv, do, 16, 8, window, sinks)
+    from train_large_model_from_scratch_b200.ops import oracle
+    q, k, v = (t.double().transpose(1, 2) for t in qkv.split([16, 8, 8], dim=2))
+    do = do.double().transpose(1, 2)
+    k, v = (t.repeat_interleave(2, dim=1) for t in (k, v))
+    seen = oracle.window_mask(T, window, sinks, "cuda")
+    p = torch.softmax((q @ k.mT / math.sqrt(d)).masked_fill(~seen, -math.inf), dim=-1)
+    dp = do @ v.mT
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_delta = H * ds.abs().sum(-1, keepdim=True) + 2.0 ** -16 * (do.abs() * (p @ v.abs())).sum(-1, keepdim=True)
+    e_ds = 1.05 * H * ds.abs() + p * (1.05 * e_delta + 2.0 ** -18 * (do.abs() @ v.abs().mT))
+    dq, e = ds @ k / math.sqrt(d), e_ds @ k.abs() / math.sqrt(d)
+    over = (got[1].double().transpose(1, 2) - dq).abs() - e - H * (dq.abs() + e)
+    assert over[:, :, :128].max().item() <= 0, [(i, over[:, :, i].max().item()) for i in range(128) if over[:, :, i].max().item() > 0][:5]
+
+
 def test_same_bits_again_and_in_a_graph():
     """o, dk and dv do not depend on the order in which blocks run (dq is reduced in hardware order); a captured call replays on
     new inputs, beside another captured call and eager ones on another stream."""

@@ -71,6 +71,22 @@ int main() {
     assert len(out) == len(cases) and not [c for c, o in zip(cases, out) if o != "0"]
 
 
+def test_rows_without_a_rest_see_a_tile_of_keys(tmp_path):
+    if shutil.which("g++") is None:
+        pytest.skip("no host compiler")
+    src, exe = tmp_path / "rest.cpp", str(tmp_path / "rest")
+    src.write_text('#include <cstdio>\n#include "window_plan.h"\nint main() { int T, W, S; while (std::scanf("%d %d %d", &T, &W, &S) == 3) '
+                   '{ std::printf("%d %d\\n", tlm::win_rest_rows(T, W, S), (int)tlm::win_few(T, W, S)); } }\n')
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", SRC, str(src), "-o", exe], check=True)
+    cases = [(T, W, S) for T in (1, 2, 127, 128, 129, 300, 1000) for W in (1, 2, 64, 127, 128, 129, 300, 1000) if W <= T
+             for S in (0, 1, 63, 64, 126, 127, 128, 300) if S <= T]
+    out = subprocess.run([exe], input="".join("%d %d %d\n" % c for c in cases), capture_output=True, text=True, check=True).stdout.split()
+    for (T, W, S), rows, few in zip(cases, map(int, out[::2]), map(int, out[1::2])):
+        keys = [sum(1 for j in range(i + 1) if i - j < W or j < S) for i in range(min(T, 400))]
+        assert rows <= T and (rows == T or rows == 128) and all(n >= 128 for n in keys[rows:]), (T, W, S, rows)
+        assert not few or max(keys) < 128, (T, W, S)
+
+
 def test_every_visible_pair_is_met_once(plan):
     rng = random.Random(0)
     sizes = [1, 2, 127, 128, 129, 255, 256, 257, 640, 1001]

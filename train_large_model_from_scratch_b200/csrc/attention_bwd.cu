@@ -83,11 +83,11 @@ template <> struct AttnBwdMaps<true> { CUtensorMap q, k, v, dout, dq; };
 // are staged in shared memory so that the [B, Hq, T] output is written as whole 128-byte lines.
 constexpr int DELTA_T = 32, DELTA_THREADS = 256;
 
-// REST: o + o_rest in place of o (see AttnFwdParams).
+// REST: o + o_rest in place of o in the first rest_rows rows, which are all or whole blocks (see AttnFwdParams).
 template <bool REST>
 __global__ void __launch_bounds__(DELTA_THREADS)
 attn_delta_kernel(const __nv_bfloat16* o, const __nv_bfloat16* o_rest, const __nv_bfloat16* dout,
-                  float* __restrict__ delta, float* __restrict__ dq_acc, int B, int T, int Hq, int hd) {
+                  float* __restrict__ delta, float* __restrict__ dq_acc, int B, int T, int Hq, int hd, int rest_rows) {
   griddep_wait();
   griddep_launch();
   extern __shared__ float delta_s[];                       // [Hq][DELTA_T + 1]
@@ -106,7 +106,8 @@ attn_delta_kernel(const __nv_bfloat16* o, const __nv_bfloat16* o_rest, const __n
   }
   const uint4* op = reinterpret_cast<const uint4*>(o + base) + sub;
   const uint4* dp = reinterpret_cast<const uint4*>(dout + base) + sub;
-  const uint4* rp = REST ? reinterpret_cast<const uint4*>(o_rest + base) + sub : nullptr;
+  const bool rest = REST && t0 < rest_rows;
+  const uint4* rp = rest ? reinterpret_cast<const uint4*>(o_rest + ((long long)b * rest_rows + t0) * Hq * hd) + sub : nullptr;
   for (int rb = 0; rb < rows; rb += 4 * slots) {          // trip count is uniform: the shuffles below need whole warps
     const int r0 = rb + slot;
     uint4 a[4], d[4], e[4];
@@ -115,7 +116,7 @@ attn_delta_kernel(const __nv_bfloat16* o, const __nv_bfloat16* o_rest, const __n
       const int rr = r0 + u * slots;
       if (rr < rows) { a[u] = op[(long long)rr * lpr]; d[u] = dp[(long long)rr * lpr]; }
       else { a[u] = make_uint4(0, 0, 0, 0); d[u] = a[u]; }
-      if (REST) e[u] = rr < rows ? rp[(long long)rr * lpr] : make_uint4(0, 0, 0, 0);
+      if (rest) e[u] = rr < rows ? rp[(long long)rr * lpr] : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -126,7 +127,7 @@ attn_delta_kernel(const __nv_bfloat16* o, const __nv_bfloat16* o_rest, const __n
         const float2 x = unpack_bf16(aw[k]), y = unpack_bf16(dw[k]);
         acc = fmaf(x.x, y.x, fmaf(x.y, y.y, acc));
       }
-      if (REST) {
+      if (rest) {
         const uint32_t ew[4] = {e[u].x, e[u].y, e[u].z, e[u].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -1044,7 +1045,8 @@ static int make_dq_map(CUtensorMap* map, const float* dq_acc, int B, int T, int 
 }
 
 // delta [B, Hq, T] and a dQ accumulator of zeros
-static int launch_delta(const void* o, const void* o_rest, const void* dout, float* delta, float* dq_acc, int B, int T, int Hq, int hd, cudaStream_t st) {
+static int launch_delta(const void* o, const void* o_rest, int rest_rows, const void* dout, float* delta, float* dq_acc, int B, int T, int Hq, int hd,
+                        cudaStream_t st) {
   // Few blocks would take longer over the zeroes than a memset (48 heads of 64, 16 rows: one block, 3 us more)
   const int delta_blocks = B * ((T + DELTA_T - 1) / DELTA_T);
   const bool fused_zero = delta_blocks >= num_sms();
@@ -1053,7 +1055,7 @@ static int launch_delta(const void* o, const void* o_rest, const void* dout, flo
     if (ce != cudaSuccess) return (int)ce;
   }
   return launch_overlapped(o_rest != nullptr ? attn_delta_kernel<true> : attn_delta_kernel<false>, dim3(delta_blocks), dim3(DELTA_THREADS),
-      (size_t)Hq * (DELTA_T + 1) * 4, st, 1, (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_rest, (const __nv_bfloat16*)dout, delta, fused_zero ? dq_acc : nullptr, B, T, Hq, hd);
+      (size_t)Hq * (DELTA_T + 1) * 4, st, 1, (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_rest, (const __nv_bfloat16*)dout, delta, fused_zero ? dq_acc : nullptr, B, T, Hq, hd, rest_rows);
 }
 
 }  // namespace tlm
@@ -1070,7 +1072,7 @@ static int attn_bwd_impl(const void* qkv, const void* o, const void* dout, const
   if (hd != 32 && hd != 64 && hd != 128) return -4;
   if (Hq % Hkv != 0) return -5;
   if ((size_t)Hq * (DELTA_T + 1) * 4 > 48 * 1024) return -6;
-  const int le = launch_delta(o, nullptr, dout, delta, dq_acc, B, T, Hq, hd, st);
+  const int le = launch_delta(o, nullptr, 0, dout, delta, dq_acc, B, T, Hq, hd, st);
   if (le) return le;
   AttnBwdMaps<false> maps;
   const int box_cols = hd == 32 && n_dst == 0 ? 32 : 64;
@@ -1139,7 +1141,7 @@ TLM_API long long tlm_attn_window_part_floats(int B, int T, int Hkv, int hd, int
   return f.chunks > 0 ? (long long)B * Hkv * (1 + f.chunks) * S * 2 * hd : 0;
 }
 
-// Backward of tlm_attn_window_fwd. strides[9] as there; out_strides[9]: of dq, dk and dv (rows of 16-byte aligned addresses). o, dout
+// Backward of tlm_attn_window_fwd. strides[9] and o_rest (may be null) as there; out_strides[9]: of dq, dk and dv (rows of 16-byte aligned addresses). o, dout
 // [B, T, Hq, hd] and lse contiguous. Scratch owned by the caller: dq_acc, delta as for tlm_attn_bwd, part (see above; may be null
 // where it takes no floats). cosT / sinT (optional, fp32 [T, hd]): the transposed rotation of dQ and dK on the way out.
 TLM_API int tlm_attn_window_bwd(const void* q, const void* k, const void* v, const long long* strides, const void* o, const void* o_rest, const void* dout,
@@ -1168,7 +1170,7 @@ TLM_API int tlm_attn_window_bwd(const void* q, const void* k, const void* v, con
   if (!e) e = make_bthd_map(&maps.dout, dout, o_strides, B, T, Hq, hd, AB_TILE);
   if (!e) e = make_dq_map(&maps.dq, dq_acc, B, T, Hq, hd);
   if (e) return e;
-  e = launch_delta(o, o_rest, dout, delta, dq_acc, B, T, Hq, hd, st);
+  e = launch_delta(o, o_rest, win_rest_rows(T, p.window, p.sinks), dout, delta, dq_acc, B, T, Hq, hd, st);
   if (e) return e;
   p.dq_acc = dq_acc; p.lse = lse; p.delta = delta; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.hd = hd;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f; p.status = status_word(); p.part = part;

@@ -25,7 +25,8 @@
 // memory, registers): scores 460 cycles, maximum 670, exponentials 1580, P V 260, and 6500 around a block's tiles. B 8, T 4096, 16 / 8
 // heads of 64, window 1024 228 us (530 TF of what is seen), 32 / 4 of 32, window 512 313 us, B 2, 16 / 4 of 128, window 2048 116 us
 // (889 TF). P is rounded to bf16 where the tensor core takes it, as in the causal form: 2^-9 of a probability on average.
-// FEW, a third one, where no row sees a tile's worth of keys: o more exactly, and its rest, for the gradients of q and k.
+// FEW, a third one, where no row sees a tile's worth of keys: o more exactly. Its rest, for the gradients of q and k, is kept there for all
+// rows, elsewhere for those of the first tile.
 #include "attention_window.h"
 
 namespace tlm {
@@ -50,9 +51,11 @@ struct AttnFwdParams {
   int hd;                  // head dim of the tensors in memory (= the kernel's HD)
   int head_group;          // heads per group of the heavy-first block order (see heavy_first_decode)
   int window, sinks;       // WIN: keys a query sees, itself included (at most T), and first keys that stay visible
-  // FEW, optional: what rounding o to bf16 took off, as bf16. The backward's delta = sum do * o is compared with do * v of single keys;
-  // where a row sees few keys they nearly cancel, and half a bf16 step of o is then much of the gradient of q and k.
+  // WIN, optional, [B, rest_rows, Hq, hd]: what o, divided by the sum of the probabilities as they were rounded, lost when it was rounded
+  // to bf16, for the first rest_rows rows of a sequence (win_rest_rows). The backward's delta = sum do * o is compared with do * v of
+  // single keys; where a row sees few keys they nearly cancel, and half a bf16 step of o is then much of the gradient of q and k.
   __nv_bfloat16* o_rest;
+  int rest_rows;
 };
 
 // WIN: q [.., Hq, hd], k and v [.., Hkv, hd]; else one map over the packed tensor
@@ -373,20 +376,46 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdMaps<WIN> tm, const AttnFwdParams
             v.z = pack_bf16(__uint_as_float(r[i + 4]) * inv, __uint_as_float(r[i + 5]) * inv);
             v.w = pack_bf16(__uint_as_float(r[i + 6]) * inv, __uint_as_float(r[i + 7]) * inv);
             *reinterpret_cast<uint4*>(out + c + i) = v;
-            if constexpr (FEW) {
-              if (p.o_rest != nullptr) {
-                auto rest = [&](int k, uint32_t w) {
-                  const float2 x = unpack_bf16(w);
-                  return pack_bf16(fmaf(__uint_as_float(r[i + k]), inv, -x.x), fmaf(__uint_as_float(r[i + k + 1]), inv, -x.y));
-                };
-                *reinterpret_cast<uint4*>(p.o_rest + (out - p.o) + c + i) = make_uint4(rest(0, v.x), rest(2, v.y), rest(4, v.z), rest(6, v.w));
-              }
-            }
             if (out2 != nullptr) *reinterpret_cast<uint4*>(out2 + c + i) = v;
           }
         }
       }
       if (t_row < p.T) p.lse[((long long)b * p.Hq + h) * p.T + t_row] = m_ref * p.scale + __logf(l_run);
+      if constexpr (WIN) {
+        if (p.o_rest != nullptr && (FEW || qt == 0)) {
+          float inv_rest = inv;
+          if (!FEW) {
+            // The first tile is its rows' only one, so its probabilities, as they were rounded, still lie where P V read them. Their sum in the
+            // loop over tiles took 75 us of 313 (8 x 4096, 32 / 8 heads of 32, window 1024), this and the stores 3.
+            float2 l2 = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < AT_BKV / 2; c += 32) {
+              uint32_t r[32];
+              tmem_ld32(t_lane + P_COL + c, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) l2 = fadd2(l2, unpack_bf16(r[i]));
+            }
+            inv_rest = 1.f / (l2.x + l2.y);
+          }
+          __nv_bfloat16* dst = p.o_rest + (((long long)b * p.rest_rows + t_row) * p.Hq + h) * p.hd;
+#pragma unroll
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(t_lane + O_COL + c, r);
+            tmem_ld_wait();
+            auto rest = [&](int k) {                            // o is rounded again, as it left
+              const float x = __uint_as_float(r[k]), y = __uint_as_float(r[k + 1]);
+              const float2 left = unpack_bf16(pack_bf16(x * inv, y * inv));
+              return pack_bf16(fmaf(x, inv_rest, -left.x), fmaf(y, inv_rest, -left.y));
+            };
+            if (t_row < p.T) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(rest(i), rest(i + 2), rest(i + 4), rest(i + 6));
+            }
+          }
+        }
+      }
     }
   }
 
@@ -454,7 +483,10 @@ TLM_API int tlm_attn_fwd_scatter(const void* qkv, void* o, float* lse, int B, in
 
 // Causal attention over a sliding window with sinks (window_plan.h) on q [B, T, Hq, hd], k and v [B, T, Hkv, hd]; strides[9]: batch,
 // token and head strides of q, k and v in elements. window <= 0 or above T: no window. o [B, T, Hq, hd], lse [B, Hq, T] contiguous;
-// o_rest: null or, over fewer than AT_BKV keys, what rounding took off o, in o's layout, for the backward.
+// o_rest: null or, for the backward, [B, rows, Hq, hd] of tlm_attn_window_rest_rows rows (see AttnFwdParams).
+TLM_API int tlm_attn_window_rest_rows(int T, int window, int sinks) {
+  return T <= 0 ? 0 : win_rest_rows(T, window > 0 && window < T ? window : T, sinks < T ? sinks : T);
+}
 TLM_API int tlm_attn_window_fwd(const void* q, const void* k, const void* v, const long long* strides, void* o, void* o_rest, float* lse, int B, int T,
                                 int Hq, int Hkv, int hd, float scale, int window, int sinks, cudaStream_t st) {
   if (hd != 32 && hd != 64 && hd != 128) return -4;
@@ -476,8 +508,8 @@ TLM_API int tlm_attn_window_fwd(const void* q, const void* k, const void* v, con
   // (0.42) and 0.0024 (0.0044) for 2 keys, 0.0035 (0.017) and 0.0025 (0.0039) for 4, 0.0027 (0.0033) and 0.0024 (0.0030) for 64, 0.0025
   // (0.0026) and 0.0024 (0.0025) for a window of 200. Taken everywhere it cost 75 us of 313 forward and 14 of 499 backward
   // (8 x 4096, 32 / 8 heads of 32, window 1024).
-  const bool few = T < AT_BKV || p.window < AT_BKV - p.sinks;
-  if (o_rest != nullptr && !few) return -6;
+  const bool few = win_few(T, p.window, p.sinks);
+  p.rest_rows = win_rest_rows(T, p.window, p.sinks);
   p.head_group = attn_head_group("TLM_ATTN_FWD_GROUP", 8LL * T * hd, 64LL << 20, B * Hq);
   if (few)
     return hd == 128 ? launch_fwd<128, true, true>(maps, p, st) : hd == 64 ? launch_fwd<64, true, true>(maps, p, st)

@@ -27,6 +27,12 @@ TLM_TILE_HD bool win_partial(int qt, int t, int W, int S) {
   return t == qt || (t * WIN_TILE < (qt + 1) * WIN_TILE - W && (t + 1) * WIN_TILE > S);
 }
 
+// No row sees a tile's worth of keys
+TLM_TILE_HD bool win_few(int T, int W, int S) { return T < WIN_TILE || W < WIN_TILE - S; }
+// Rows of which the backward wants o more exactly than bf16 holds it (AttnFwdParams::o_rest), because they see few keys: all of them, or
+// those of the first tile: behind it every row sees 128 keys or more.
+TLM_TILE_HD int win_rest_rows(int T, int W, int S) { return win_few(T, W, S) ? T : WIN_TILE; }
+
 // ---- backward: a block takes KV tile j and the query tiles of its window, j .. win_last_q. What sees the tile only as sinks, the
 // query tiles after that ("far"), is cut into pieces of `chunk` query tiles that are blocks of their own: one tile with all of
 // them would take as long as the sequence is.

@@ -138,12 +138,16 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 def _window_fwd(q: int, k: int, v: int, strides, B: int, T: int, n_q: int, n_kv: int, hd: int, window: int, sinks: int, device,
                 rest: bool):
     o = torch.empty((B, T, n_q, hd), dtype=torch.bfloat16, device=device)
-    rest = rest and min(T, (window or T) + sinks) < 128             # no row sees a tile of keys
-    o_rest = torch.empty((B, T, n_q, hd), dtype=torch.bfloat16, device=device) if rest else None
+    o_rest = torch.empty((B, _rest_rows(T, min(window, T), min(sinks, T)), n_q, hd), dtype=torch.bfloat16, device=device) if rest else None
     lse = torch.empty((B, n_q, T), dtype=torch.float32, device=device)
     native._check(native.lib().tlm_attn_window_fwd(q, k, v, strides, o.data_ptr(), native._ptr(o_rest), lse.data_ptr(), B, T, n_q,
                                                    n_kv, hd, 1.0 / math.sqrt(hd), min(window, T), min(sinks, T), native._stream()), "attn_window_fwd")
     return o, lse, o_rest
+
+
+@functools.lru_cache(maxsize=1024)
+def _rest_rows(T: int, window: int, sinks: int) -> int:
+    return native.lib().tlm_attn_window_rest_rows(T, window, sinks)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -178,7 +182,7 @@ def _packed(qkv: torch.Tensor, n_q: int, n_kv: int):
 def window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int, rest: bool = False):
     """Causal attention of `q [B, T, Hq, hd]` over `k`, `v [B, T, Hkv, hd]` (bf16, hd 32 / 64 / 128, strided) where a query sees
     `window` keys, itself included (0: all), and the first `sinks`. -> o `[B, T, Hq, hd]` bf16, lse `[B, Hq, T]` fp32 and, with `rest`,
-    what rounding took off o (bf16, for the backward; None over many keys)."""
+    what rounding took off o in the first rows, or in all where none sees many keys (bf16, for the backward)."""
     q, k, v = _tiled(q), _tiled(k), _tiled(v)
     B, T, n_q, hd = q.shape
     strides = native._LL9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])

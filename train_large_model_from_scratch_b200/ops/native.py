@@ -85,6 +85,7 @@ _SIGS = {
     "tlm_attn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P]),
     "tlm_attn_bwd_scatter": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "tlm_attn_window_fwd": (_I, [_P] * 7 + [_I] * 5 + [_F, _I, _I, _P]),
+    "tlm_attn_window_rest_rows": (_I, [_I] * 3),
     "tlm_attn_window_part_floats": (_LL, [_I] * 6),
     "tlm_attn_window_bwd": (_I, [_P] * 15 + [_I] * 5 + [_F, _P, _P, _I, _I, _P]),
     "tlm_qk_rotary": (_I, [_P] * 5 + [_LL, _P, _I, _P, _P] + [_I] * 5 + [_F, _F, _I, _I, _P]),
