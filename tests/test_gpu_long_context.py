@@ -89,6 +89,24 @@ def test_one_node_is_the_operators_in_a_row():
     assert ((dx[:, :, :n_q].double() - dx2[:, :, :n_q].double()).norm() <= 4 * H * dx2[:, :, :n_q].double().norm()).item()
 
 
+def test_a_tangent_is_refused():
+    """The kernels know nothing of forward-mode derivatives: a tangent is refused, not dropped; other calls beside it run."""
+    import torch.autograd.forward_ad as fwad
+    from train_large_model_from_scratch_b200.ops import functional as F_ops
+    qkv, _, w = _case(1, 40, 4, 2, 64, True)
+    pos, freq = torch.arange(40, device="cuda"), torch.ones(32, dtype=torch.float64, device="cuda")
+    plain = F_ops.rotary(qkv, pos, freq)
+    for call in (lambda x: F_ops.rotary(x, pos, freq), lambda x: F_ops.qk_norm_rotary(x, 4, *[t.detach() for t in w], pos, freq),
+                 lambda x: F_ops.attention_packed(x, 4, 2, window=7), lambda x: F_ops.rotary_attention(x, 4, 2, pos, freq, window=7),
+                 lambda x: F_ops.window_attention(x[:, :, :4], x[:, :, 4:6], x[:, :, 6:], 7)):
+        with fwad.dual_level():
+            with pytest.raises(RuntimeError, match="jvp"):
+                call(fwad.make_dual(qkv, torch.ones_like(qkv)))
+            with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                call(fwad.make_dual(qkv, torch.ones_like(qkv)))
+            assert torch.equal(F_ops.rotary(qkv, pos, freq), plain)
+
+
 def _models(over):
     from train_large_model_from_scratch_b200.models import GPT
     from train_large_model_from_scratch_b200.models.modules.init import clear_init_cache

@@ -180,6 +180,36 @@ def test_a_negative_eps_is_refused(eps):
         Fo.rotary_attention(qkv, 2, 1, pos, freq, norm_weights=(w, w), eps=eps)
 
 
+def _with_tangent(call, x, *others):
+    """`call` on `x` with a tangent, under forward-mode derivatives; the tangent of the result."""
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level():
+        return fwad.unpack_dual(call(fwad.make_dual(x, torch.ones_like(x)), *others)).tangent
+
+
+def test_a_tangent_is_followed_or_refused(monkeypatch):
+    """The torch path differentiates forward; the kernels (stood in for here) cannot, and say so."""
+    from train_large_model_from_scratch_b200.ops import attention_cuda, native
+    qkv, pos, freq, w = _randn(1, 4, 4, 32), torch.arange(4), torch.ones(16, dtype=torch.float64), torch.ones(32)
+    calls = [(lambda x: Fo.rotary(x, pos, freq), qkv), (lambda x: Fo.qk_norm_rotary(x, 2, w, w, pos, freq), qkv),
+             (lambda x: Fo.qk_norm_rotary(qkv, 2, x, w, pos, freq), w), (lambda x: Fo.attention_packed(x, 2, 1, window=2), qkv),
+             (lambda x: Fo.window_attention(qkv[:, :, :2], x, qkv[:, :, 3:], 2), qkv[:, :, 2:3])]
+    for call, x in calls:
+        t, h = _with_tangent(call, x), 1e-2
+        # the third derivative of a softmax or a norm of size 1, times h^2 / 6, and 2^-24 / h of the results
+        torch.testing.assert_close(t, (call(x + h) - call(x - h)) / (2 * h), rtol=1e-2, atol=1e-3)
+    monkeypatch.setattr(Fo, "_use_native", lambda *a: True)
+    monkeypatch.setattr(native, "qk_rotary", lambda x, *a, **k: x.clone())
+    monkeypatch.setattr(attention_cuda, "window_fwd", lambda q, *a, **k: (q.clone(), q.new_zeros(()), None))
+    monkeypatch.setattr(attention_cuda, "window_fwd_packed", lambda x, n_q, *a, **k: (x[:, :, :n_q].clone(), x.new_zeros(()), None))
+    grads = qkv.clone().requires_grad_()
+    calls += [(lambda x: Fo.qk_norm_rotary(grads, 2, x, w, pos, freq), w), (lambda x: Fo.rotary_attention(x, 2, 1, pos, freq), qkv),
+              (lambda x: Fo.rotary_attention(grads, 2, 1, pos, freq, norm_weights=(w, x)), w)]
+    for call, x in calls:
+        with pytest.raises(RuntimeError, match="jvp"):
+            _with_tangent(call, x)
+
+
 def test_config():
     flags = ["--rope_variant", "standard", "--qk_norm", "--rope_layout", "interleaved", "--rope_fraction", "0.5", "--rope_scaling", "yarn",
              "--rope_scaling_factor", "4", "--attn_window", "64", "--attn_sinks", "4"]

@@ -17,6 +17,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import oracle
 from . import native
@@ -333,12 +334,20 @@ def attention_packed(qkv: torch.Tensor, n_q: int, n_kv: int, causal: bool = True
     if qkv.dim() != 4 or qkv.shape[2] != n_q + 2 * n_kv:
         raise ValueError(f"qkv has to be [B, T, {n_q + 2 * n_kv}, hd], not {tuple(qkv.shape)}")
     _check_window(qkv, n_q, n_kv, window, sinks)
-    if not (qkv.requires_grad and torch.is_grad_enabled()):
+    if not _needs_node(qkv):
         return _window_packed_fwd(qkv, n_q, n_kv, window, sinks)[0]
     return _WindowPacked.apply(qkv, (n_q, n_kv, window, sinks))
 
 
 # --------------------------------------------------------------------------- attention over a sliding window with sinks
+def _needs_node(x, *others) -> bool:
+    """Whether a call has to be one of autograd's: gradients of it are wanted, or it runs on the GPU under forward-mode derivatives,
+    of which the kernels know nothing (they would drop a tangent; a node refuses it)."""
+    if torch.is_grad_enabled() and (x.requires_grad or any(t.requires_grad for t in others)):
+        return True
+    return forward_ad._current_level >= 0 and _use_native(x)
+
+
 def _heads_of(qkv, n_q, n_kv):
     return qkv[:, :, :n_q], qkv[:, :, n_q:n_q + n_kv], qkv[:, :, n_q + n_kv:]
 
@@ -430,7 +439,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if q.dtype != k.dtype or q.dtype != v.dtype:
         raise ValueError(f"q, k and v of one type expected, not {q.dtype}, {k.dtype}, {v.dtype}")
     _check_window(q, q.shape[2], k.shape[2], window, sinks, k, v)
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    if not _needs_node(q, k, v):
         if _use_native(q):
             return attention_cuda.window_fwd(q, k, v, window, sinks)[0]
         return _attn_fwd_ref(q, k, v, True, window, sinks)[0].to(q.dtype).contiguous()
@@ -499,14 +508,15 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, int
     contiguous)."""
     x, positions, inv_freq = _check_rotary(x, positions, inv_freq)
     turn = _Turn(positions, inv_freq, interleaved, scale)
-    return _Rotary.apply(x, turn) if x.requires_grad and torch.is_grad_enabled() else _turn(x, turn)
+    return _Rotary.apply(x, turn) if _needs_node(x) else _turn(x, turn)
 
 
 def _anchors(x, weights):
     """The weights as inputs of a node, only where the node would have no differentiable input without them: their gradients go to
     `main_grad`, and a parameter that is an input ties the node to the stream on which the parameter was first used (a backward
-    pass cannot then be captured while an older graph of the same parameters lives)."""
-    return () if x.requires_grad or weights is None else weights
+    pass cannot then be captured while an older graph of the same parameters lives). And under forward-mode derivatives, which the
+    node refuses for inputs with a tangent."""
+    return () if weights is None or (x.requires_grad and forward_ad._current_level < 0) else weights
 
 
 class _QkNormRotary(torch.autograd.Function):
@@ -569,7 +579,7 @@ def qk_norm_rotary(x: torch.Tensor, n_q: int, q_weight: torch.Tensor, k_weight: 
     _check_norm(x, eps, q_weight, k_weight)
     weights = (q_weight, k_weight)
     args = (weights, int(n_q), float(eps), _Turn(positions, inv_freq, interleaved, scale))
-    if torch.is_grad_enabled() and (x.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+    if _needs_node(x, q_weight, k_weight):
         return _QkNormRotary.apply(x, args, *_anchors(x, weights))
     return _qk_norm_fwd(x, *args)
 
