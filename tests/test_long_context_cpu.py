@@ -271,6 +271,13 @@ def test_model_gradients_against_differences(kw):
         assert abs((vals[0] - vals[1]) / (2 * h) / norm ** 2 - 1) < 0.02
 
 
+@pytest.mark.parametrize("kw", [dict(qk_norm=True), dict(attn_window=4, qk_norm=True, tied_lm_head=False), dict(rope_fraction=0.5)])
+def test_exact_number_of_parameters(kw):
+    from train_large_model_from_scratch_b200.utils.model import count_exact_params
+    cfg = _tiny(**kw)
+    assert count_exact_params(cfg) == sum(p.numel() for p in GPT(cfg, device="cpu").parameters())
+
+
 def test_flop_count_of_a_window():
     full, part = (GPT(_tiny(attn_window=w), device="cpu").get_exact_flops_per_fwd_bwd(1, 32) for w in (0, 4))
     assert part < full

@@ -44,6 +44,8 @@ def count_exact_params(c: ModelConfig, ep_size: int = 1) -> int:
     """Exact number of parameters held by one rank (experts divided by `ep_size`)."""
     H, hd = c.hidden_size, c.hidden_size // c.num_attention_heads
     attn = H * c.num_attention_heads * hd + 2 * H * c.num_key_value_heads * hd + H * H
+    if c.qk_norm:
+        attn += 2 * hd
     if c.use_moe:
         ffn = H * c.num_experts + (c.num_experts // ep_size) * 3 * H * c.moe_intermediate_size
     else:
