@@ -283,6 +283,17 @@ def test_flop_count_of_a_window():
     assert part < full
 
 
+@pytest.mark.parametrize("T,W,S", [(32, 4, 0), (32, 4, 3), (32, 4, 14), (32, 4, 28), (32, 4, 1000), (32, 1, 31), (32, 31, 1), (32, 32, 5), (31, 7, 11)])
+def test_flop_count_is_that_of_the_visible_pairs(T, W, S):
+    """Attention's part: 14 multiplications and additions for each pair, head and element; a triangle of n rows counts as n^2 / 2 pairs, as in
+    the causal form: W / 2 for the window's, one of S for the sinks'."""
+    count = lambda **kw: GPT(_tiny(**kw), device="cpu").get_exact_flops_per_fwd_bwd(1, T)  # noqa: E731
+    layers, hidden = 2, 32
+    causal, pairs = T * T / 2, int(oracle.window_mask(T, W, S).sum())
+    got = (count(attn_window=W, attn_sinks=S) - count()) / (14 * layers * hidden) + causal
+    assert abs(got - pairs) <= (min(W, T) + min(S, T - W)) / 2 + 1e-6, (got, pairs)
+
+
 def test_ranks_of_a_sequence_group_agree():
     """sep = 2 (heads and sequence exchanged) against one rank, all options on: same losses and gradient norms."""
     tmp = tempfile.mkdtemp(prefix="tlm_test_")

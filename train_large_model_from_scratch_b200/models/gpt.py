@@ -294,9 +294,10 @@ class GPT(nn.Module):
         hd = D // c.num_attention_heads
         proj = 2 * B * T * D * (c.num_attention_heads * hd + 2 * c.num_key_value_heads * hd + D)
         attn = 4 * B * T * T * D / 2
-        if 0 < c.attn_window < T:                    # whole windows, the rows before the first one, and the sinks in front of them
-            W, late = c.attn_window, T - c.attn_window
-            attn = 4 * B * D * (W * W / 2 + late * (W + min(c.attn_sinks, late / 2)))
+        if 0 < c.attn_window < T:                    # the rows before the first whole window, whole windows, and the sinks in front of
+            W, late = c.attn_window, T - c.attn_window             # them: one more sink each row until all are seen
+            sinks = min(c.attn_sinks, late)
+            attn = 4 * B * D * (W * W / 2 + late * W + sinks * late - sinks * sinks / 2)
         if self.use_moe:
             ffn = 2 * B * T * D * c.num_experts + c.num_experts_per_tok * 6 * B * T * D * c.moe_intermediate_size
         else:
