@@ -180,6 +180,12 @@ def test_a_negative_eps_is_refused(eps):
         Fo.rotary_attention(qkv, 2, 1, pos, freq, norm_weights=(w, w), eps=eps)
 
 
+def test_a_window_without_a_kernel_is_refused_when_the_model_is_built():
+    with pytest.raises(ValueError, match="head dim 8"):
+        GPT(_tiny(attn_window=4), device="cuda")
+    GPT(_tiny(attn_window=4), device="cpu")
+
+
 def _with_tangent(call, x, *others):
     """`call` on `x` with a tangent, under forward-mode derivatives; the tangent of the result."""
     import torch.autograd.forward_ad as fwad

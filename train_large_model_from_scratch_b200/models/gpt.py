@@ -100,6 +100,9 @@ class GPT(nn.Module):
         if compute_dtype is None:
             compute_dtype = torch.bfloat16 if self.device.type == "cuda" else torch.float32
         self.compute_dtype = compute_dtype
+        if config.attn_window > 0 and self.device.type == "cuda" and compute_dtype == torch.bfloat16 \
+                and config.head_dim not in F_ops.WINDOW_HEAD_DIMS:
+            raise ValueError(f"attn_window with head dim {config.head_dim}: the window kernels have {F_ops.WINDOW_HEAD_DIMS}")
         self.use_moe = config.use_moe
         dev = self.device
         self.wte = TextEmbedding(config.vocab_size, config.hidden_size, device=dev)

@@ -370,12 +370,15 @@ def _check_window(x, n_q, n_kv, window, sinks, *others) -> None:
         raise ValueError(f"window {window}, sinks {sinks}: neither may be negative, and sinks need a window")
     _check_device(x, *others)
     if not window_attention_ok(x):
-        raise ValueError(f"head dim {x.shape[3]}: the window kernels have 32, 64 and 128")
+        raise ValueError(f"head dim {x.shape[3]}: the window kernels have {WINDOW_HEAD_DIMS}")
+
+
+WINDOW_HEAD_DIMS = (32, 64, 128)
 
 
 def window_attention_ok(x: torch.Tensor) -> bool:
     """Whether `window_attention` has a kernel for heads like `x`'s (off the GPU it always has)."""
-    return not _use_native(x) or x.shape[3] in (32, 64, 128)
+    return not _use_native(x) or x.shape[3] in WINDOW_HEAD_DIMS
 
 
 class _Window(torch.autograd.Function):
