@@ -216,6 +216,20 @@ def test_a_tangent_is_followed_or_refused(monkeypatch):
             _with_tangent(call, x)
 
 
+def test_derivatives_by_the_frequencies_are_refused():
+    import torch.autograd.forward_ad as fwad
+    qkv, pos, w = _randn(1, 4, 4, 8), torch.arange(4), torch.ones(8)
+    freq = torch.ones(4, dtype=torch.float64, requires_grad=True)
+    calls = (lambda f: Fo.rotary(qkv, pos, f), lambda f: Fo.qk_norm_rotary(qkv, 2, w, w, pos, f), lambda f: Fo.rotary_attention(qkv, 2, 1, pos, f))
+    for call in calls:
+        with pytest.raises(ValueError, match="constant"):
+            call(freq)
+        with torch.no_grad():
+            call(freq)
+        with fwad.dual_level(), pytest.raises(ValueError, match="constant"):
+            call(fwad.make_dual(freq.detach(), torch.ones(4, dtype=torch.float64)))
+
+
 def test_config():
     flags = ["--rope_variant", "standard", "--qk_norm", "--rope_layout", "interleaved", "--rope_fraction", "0.5", "--rope_scaling", "yarn",
              "--rope_scaling_factor", "4", "--attn_window", "64", "--attn_sinks", "4"]

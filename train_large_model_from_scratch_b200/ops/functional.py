@@ -460,6 +460,8 @@ def _check_rotary(x, positions, inv_freq) -> tuple[torch.Tensor, torch.Tensor, t
         raise ValueError(f"positions have to be int64 [{T}] or [{B}, {T}], not {positions.dtype} {tuple(positions.shape)}")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 1 <= inv_freq.numel() <= hd // 2:
         raise ValueError(f"inv_freq has to be float64 with 1 to {hd // 2} frequencies, not {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    if (torch.is_grad_enabled() and inv_freq.requires_grad) or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(inv_freq).tangent is not None):
+        raise ValueError("inv_freq is a constant: no derivative by it is taken")
     _check_device(x, positions, inv_freq)
     if positions.dim() == 2 and positions.shape[0] == 1:
         positions = positions[0]
