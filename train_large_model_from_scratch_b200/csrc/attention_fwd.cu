@@ -23,7 +23,7 @@
 // that the window and the sinks leave, the row's own first: its maximum is then finite, whatever is hidden later. Hidden scores become
 // -infinity before anything looks at them. What bounds it is the way from tile to tile of the two blocks an SM has room for (tensor
 // memory, registers): scores 460 cycles, maximum 670, exponentials 1580, P V 260, and 6500 around a block's tiles. B 8, T 4096, 16 / 8
-// heads of 64, window 1024 228 us (530 TF of what is seen), 32 / 4 of 32, window 512 313 us, B 2, 16 / 4 of 128, window 2048 116 us
+// heads of 64, window 1024 228 us (530 TF of what is seen), 32 / 4 of 32, window 512 314 us, B 2, 16 / 4 of 128, window 2048 116 us
 // (889 TF). P is rounded to bf16 where the tensor core takes it, as in the causal form: 2^-9 of a probability on average.
 // FEW, a third one, where no row sees a tile's worth of keys: o more exactly. Its rest, for the gradients of q and k, is kept there for all
 // rows, elsewhere for those of the first tile.
@@ -92,7 +92,8 @@ struct AttnFwdSmem {
 constexpr float RESCALE_LOG2 = 8.0f;
 
 // 2^x for x <= 127 on the FMA pipe: x = n + f with n the nearest integer (the sum with 1.5 * 2^23 + 127 leaves n + 127 in the low bits), a
-// polynomial of degree 3 for 2^f on [-1/2, 1/2] (minimax, off by 7.5e-5, a fiftieth of half a bf16 step), times 2^n.
+// polynomial of degree 3 for 2^f on [-1/2, 1/2] (minimax, off by 7.5e-5, a fiftieth of half a bf16 step), times 2^n. The row's sum adds up
+// what P V is given, so it and lse are off by at most as much (7.5e-5, where such a pair holds all of a row's weight).
 // Below -126, -infinity included, that is 0.99993 * 2^-126; less 2^-126 it is nearer to zero than to any bf16, and so a hidden key's
 // probability is. NaN stays NaN.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {

@@ -1,4 +1,4 @@
-// What the window attention's forward (attention_window_fwd.cu) and backward (attention_bwd.cu) share.
+// What the window attention's forward (attention_fwd.cu) and backward (attention_bwd.cu) share.
 #pragma once
 #include "common.cuh"
 #include "window_plan.h"

@@ -433,7 +433,8 @@ class _WindowPacked(torch.autograd.Function):
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0) -> torch.Tensor:
     """Causal GQA attention of `q [B, T, Hq, hd]` over `k`, `v [B, T, Hkv, hd]` -> `[B, T, Hq, hd]`: key j is visible to query i iff
     j <= i and (i - j < window or j < sinks); `window` 0: no window. The three may be views of one another's storage or of a
-    packed tensor; rows that are no whole 16-byte pieces apart are copied first. bf16 on the GPU with head dims 32, 64, 128.
+    packed tensor; rows that are no whole 16-byte pieces apart are copied first. bf16 on the GPU with head dims 32, 64, 128; other
+    types there, and any off it, take a torch expression over all T x T scores.
     Hidden keys and values may hold anything finite, for the output and the gradients of what does not see them. Inputs have to be
     finite where a row's 128 neighbours look: a hidden key's weight is exactly zero, but zero times an infinite or NaN value is
     NaN."""
@@ -507,8 +508,9 @@ class _Rotary(torch.autograd.Function):
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
-    """Every head of `x [B, T, H, hd]` turned by its token's position: `positions` int64 `[T]` or `[B, T]` (any values; an angle is off by
-    a few 2^-53 of itself), `inv_freq` and `scale` from `oracle.rotary_frequencies`. The first `2 * len(inv_freq)` elements of a head
+    """Every head of `x [B, T, H, hd]` turned by its token's position: `positions` int64 `[T]` or `[B, T]` (any values; the product with a
+    frequency is off by a few 2^-53 of itself, and what whole turns leave of it is rounded to 32 bits: 2e-7 radians), `inv_freq` and
+    `scale` from `oracle.rotary_frequencies`. The first `2 * len(inv_freq)` elements of a head
     turn, in pairs (i, i + len(inv_freq)) or, `interleaved`, (2 i, 2 i + 1); the rest passes. A new tensor; `x` may be a view (rows
     contiguous)."""
     x, positions, inv_freq = _check_rotary(x, positions, inv_freq)
