@@ -777,6 +777,7 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdMaps<WIN> tm, const AttnBwdParams
           if ((uint32_t)(2 * i + 1 - first) >= width) dd[i] &= 0x0000ffffu;
         }
         __syncwarp();
+        tmem_st_wait();                                        // the first stores; nothing orders two to the same place
         tmem_st16(t_s + 16, dd);
         store_ds();
       }
